@@ -96,7 +96,6 @@ def prepare(case, seed):
         s["ids"] = (torch.exp(uniform(n) * math.log(v + 1)).long() - 1).clamp(0, v - 1)
         s["scale"] = math.sqrt(d)
         if case["train"]:
-            s["weight"].requires_grad_()
             s["d_out"] = normal(n, d)
         return s
     if case["op"] == "log_probs":
@@ -108,7 +107,6 @@ def prepare(case, seed):
             s["unavailable"] = uniform(r, a) < 0.25
             s["unavailable"].scatter_(1, s["taken"][:, None], False)
         if case["train"]:
-            s["logits"].requires_grad_()
             s["d_log_prob"], s["d_entropy"] = normal(r, kind=torch.float32), normal(r, kind=torch.float32, scale=0.01)
         return s
     b, t, d = case["batch"], case.get("time", 1), case["dim"]
@@ -124,8 +122,6 @@ def prepare(case, seed):
     s["starts"] = uniform(b, t) < 1.0 / 128 if case["resets"] else None
     s["ends"] = (uniform(b) * (t + 1)).int() if case["lengths"] else None
     if case["train"]:
-        for k in ("x", "g", "h0"):
-            s[k].requires_grad_()
         s["d_h"], s["d_last"] = normal(b, t, d), normal(b, d, kind=torch.float32)
     return s
 
@@ -138,29 +134,33 @@ def run(state):
 
 
 def _own(s):
+    """The calls of a learner, which runs its backward pass explicitly as the framework's own learners do."""
     import pearl_amd
     if s["op"] == "embed":
         out = pearl_amd.embed_tokens(s["weight"], s["ids"], scale=s["scale"])
         if not s["train"]:
             return {"out": out}
-        return {"out": out, "d_weight": torch.autograd.grad(out, s["weight"], s["d_out"])[0]}
+        return {"out": out, "d_weight": pearl_amd.embed_tokens_grad(s["d_out"], s["ids"], s["vocab"], scale=s["scale"])}
+    logit = s.get("gate") == "logit"
     if s["op"] == "step":
-        h, last = pearl_amd.gated_recurrence_step(s["x"], s["g"], s["h0"], gate_logits=s["gate"] == "logit")
+        h, last = pearl_amd.gated_recurrence_step(s["x"], s["g"], s["h0"], gate_logits=logit)
         return {"h": h, "last": last}
     if s["op"] == "recurrence":
-        h, last = pearl_amd.gated_recurrence(s["x"], s["g"], s["h0"], resets=s["starts"], lengths=s["ends"],
-                                             gate_logits=s["gate"] == "logit", reverse=s["reverse"])
+        how = {"resets": s["starts"], "lengths": s["ends"], "gate_logits": logit, "reverse": s["reverse"]}
         if not s["train"]:
+            h, last = pearl_amd.gated_recurrence(s["x"], s["g"], s["h0"], **how)
             return {"h": h, "last": last}
-        dx, dg, d0 = torch.autograd.grad((h, last), (s["x"], s["g"], s["h0"]), (s["d_h"], s["d_last"]))
+        h, last, kept = pearl_amd.gated_recurrence(s["x"], s["g"], s["h0"], keep=True, **how)
+        dx, dg, d0 = pearl_amd.gated_recurrence_grad(s["x"], s["g"], kept, s["d_h"], s["d_last"], **how)
         return {"h": h, "last": last, "d_x": dx, "d_g": dg, "d_h0": d0}
     o = pearl_amd.action_log_probs(s["logits"], s["taken"], s["unavailable"], temperature=s["temperature"], top=s["top"])
+    out = {"log_prob": o.log_prob, "entropy": o.entropy}
     if s["train"]:
-        dl, = torch.autograd.grad((o.log_prob, o.entropy), s["logits"], (s["d_log_prob"], s["d_entropy"]))
-        return {"log_prob": o.log_prob, "entropy": o.entropy, "d_logits": dl}
+        out["d_logits"] = pearl_amd.action_log_probs_grad(o, s["logits"], s["taken"], s["d_log_prob"], s["d_entropy"],
+                                                          s["unavailable"], temperature=s["temperature"])
     if s["top"]:
-        return {"log_prob": o.log_prob, "entropy": o.entropy, "top": o.top_actions, "top_log_prob": o.top_log_probs}
-    return {"log_prob": o.log_prob, "entropy": o.entropy}
+        out.update({"top": o.top_actions, "top_log_prob": o.top_log_probs})
+    return out
 
 
 def _plain_embed(s):
