@@ -44,7 +44,9 @@ typedef enum pa_dtype {
   PA_I64 = 1,
   PA_I32 = 2,
   PA_U8 = 3, /* torch.bool / torch.uint8 */
-  PA_F64 = 4
+  PA_F64 = 4,
+  PA_BF16 = 5, /* the token-policy operators only (pa_embed_tokens .. pa_action_log_probs_grad) */
+  PA_F16 = 6
 } pa_dtype;
 
 const char* pa_last_error(void);
@@ -1049,6 +1051,100 @@ int pa_linreg_sigma(const float* features, int32_t ldf, const float* inv_A, int3
 /* out[B, nl + nr] = left[B, nl] || right[B, nr]   (q_value_networks.py:166-168 torch.cat) */
 int pa_concat_cols(const float* left, int32_t ldl, const float* right, int32_t ldr, float* out,
                    int32_t B, int32_t nl, int32_t nr, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Token policies: embedding, gated linear recurrence, log probabilities.     */
+/* Stateless; every pointer is device memory on `device`, which need not be   */
+/* the current one, and everything runs on `stream`.  Rows may start at any   */
+/* element (no 16-byte alignment is assumed).  Scratch is the caller's, one   */
+/* per call in flight; its contents need no initialisation.                   */
+/* ------------------------------------------------------------------------ */
+/* out[i, :] = scale * weight[tokens[i], :], rounded once: one_hot_action_representation_module.py:27-34
+ * followed by a dense layer, without the one-hot matrix.  dtype (weight and out): PA_F32 / PA_BF16 /
+ * PA_F16; tokens PA_I32 / PA_I64; weight rows ldw elements apart, out contiguous [n][dim].  Token -1
+ * means none: a row of zeros, no gradient.  Any other token outside [0, vocab) gives a row of NaN. */
+int pa_embed_tokens(const void* weight, int32_t dtype, int64_t ldw, int64_t vocab, int32_t dim,
+                    const void* tokens, int32_t token_dtype, int64_t n, float scale, void* out,
+                    int32_t device, void* stream);
+/* d_weight [vocab][dim] (written whole) = scale * sum over i with tokens[i] = v of d_out[i, :]: fp32
+ * sums in index order, rounded once, the same bits for the same inputs.  scratch:
+ * pa_embed_tokens_grad_scratch bytes, 256-byte aligned. */
+int64_t pa_embed_tokens_grad_scratch(int64_t n, int32_t dim);
+int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ldd, const void* tokens,
+                         int32_t token_dtype, int64_t n, float scale, int64_t vocab, int32_t dim,
+                         void* d_weight, void* scratch, int32_t device, void* stream);
+
+/* Gated linear recurrence over histories (pa_ppo_gae is its one-channel fp32 form):
+ *   gate_logits = 0:  h_t = g_t h_{t-1} + x_t
+ *   gate_logits = 1:  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(g_t)
+ * The state is fp32; h is rounded to the input's type.  Strides in elements, channels adjacent. */
+typedef struct pa_recurrence_args {
+  int32_t device;
+  int32_t dtype;              /* of x, h, d_h, d_x: PA_F32 / PA_BF16 / PA_F16               */
+  int32_t gate_dtype;         /* of gate, d_gate: the same, or PA_F32                       */
+  int32_t gate_logits;
+  int32_t reverse;            /* 1: from the last step to the first                         */
+  int32_t D;                  /* channels                                                   */
+  int64_t B, T;               /* histories, steps                                           */
+  const void* x;
+  int64_t x_b, x_t;
+  const void* gate;
+  int64_t gate_b, gate_t;
+  const float* h0;            /* [B][D]; NULL: zeros                                        */
+  const uint8_t* resets;      /* 1: the step ignores the state before it; NULL: none        */
+  int64_t resets_b, resets_t;
+  const int32_t* lengths;     /* [B], clamped to [0, T]; NULL: T.  Steps behind the end: h and
+                                 gradients are 0, whatever x and gate hold there            */
+  void* h;                    /* [B][T][D]                                                  */
+  float* last;                /* [B][D] state behind the last step; may be h0 when T = 1; NULL: not wanted */
+  float* carries;             /* pa_gated_recurrence_carries floats: written by the forward pass for
+                                 the gradient, read by it; NULL in a forward pass alone     */
+  void* scratch;              /* pa_gated_recurrence_scratch bytes, 256-byte aligned        */
+  /* pa_gated_recurrence_grad: */
+  const void* d_h;            /* NULL: zeros                                                */
+  int64_t d_h_b, d_h_t;
+  const float* d_last;        /* [B][D]; NULL: zeros                                        */
+  void* d_x;                  /* [B][T][D]                                                  */
+  void* d_gate;               /* [B][T][D]                                                  */
+  float* d_h0;                /* [B][D]; NULL: not wanted                                   */
+} pa_recurrence_args;
+int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D, int32_t dtype);
+int64_t pa_gated_recurrence_carries(int64_t B, int64_t T, int32_t D);
+int pa_gated_recurrence(const pa_recurrence_args* args, void* stream);
+int pa_gated_recurrence_grad(const pa_recurrence_args* args, void* stream);
+
+/* Log probability of given actions, entropy and best alternatives of softmax(logits / temperature)
+ * over the available actions (actor_networks.py:155-176 in logarithms, any number of actions).
+ * Unavailable: mask 1, or a logit of -inf.  A row without an available action: log_prob -inf, entropy
+ * 0, alternatives -1 / -inf, gradient 0.  Action -1: none given, log_prob 0; any other action outside
+ * [0, A): NaN.  Alternatives in falling order, equal logits by index. */
+typedef struct pa_log_probs_args {
+  int32_t device;
+  int32_t dtype;              /* of logits, d_logits: PA_F32 / PA_BF16 / PA_F16             */
+  int32_t action_dtype;       /* PA_I32 / PA_I64                                            */
+  int32_t A;
+  int64_t rows;
+  const void* logits;
+  int64_t ld;                 /* elements between rows                                      */
+  const void* actions;        /* [rows]                                                     */
+  const uint8_t* mask;        /* 1 = unavailable; NULL: all are available                   */
+  int64_t ldm;                /* bytes between rows; 0: one row for all                     */
+  float temperature;
+  int32_t top;                /* 0 .. 64 alternatives                                       */
+  float* log_prob;            /* [rows]                                                     */
+  float* entropy;             /* [rows]                                                     */
+  float* stats;               /* [rows][3]: written for the gradient, read by it; NULL: not wanted */
+  int64_t* top_actions;       /* [rows][top]                                                */
+  float* top_log_probs;       /* [rows][top]                                                */
+  void* scratch;              /* pa_action_log_probs_scratch bytes, 256-byte aligned        */
+  /* pa_action_log_probs_grad: */
+  const float* d_log_prob;    /* [rows]; NULL: zeros                                        */
+  const float* d_entropy;     /* [rows]; NULL: zeros                                        */
+  void* d_logits;             /* [rows][A]                                                  */
+} pa_log_probs_args;
+int64_t pa_action_log_probs_scratch(int64_t rows, int32_t A, int32_t dtype, int32_t top);
+int pa_action_log_probs(const pa_log_probs_args* args, void* stream);
+int pa_action_log_probs_grad(const pa_log_probs_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Diagnostics: single-kernel entry points so the GPU test-suite can localise */

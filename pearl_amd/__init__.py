@@ -22,6 +22,11 @@ from .policy_learners.contextual_bandits import (NeuralLinearBandit, SquareCBExp
                                                  UCBExploration)
 from .action_representation_modules import OneHotActionTensorRepresentationModule  # noqa: F401
 from .utils.instantiations.spaces import BoxActionSpace, DiscreteActionSpace  # noqa: F401
+from .neural_networks.common.token_ops import (embed_tokens, embed_tokens_grad, gated_recurrence,  # noqa: F401
+                                               gated_recurrence_grad, gated_recurrence_step)
+from .neural_networks.sequential_decision_making.action_log_probs import (ActionLogProbs,  # noqa: F401
+                                                                          action_log_probs,
+                                                                          action_log_probs_grad)
 from .vector_env import BatchedActionResult, BatchedEnvironment, VectorEnvFeeder  # noqa: F401
 
 __version__ = "0.1.0"

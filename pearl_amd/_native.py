@@ -24,7 +24,7 @@ PA_ERR_UNSUPPORTED = -4
 PA_ERR_NOMEM = -5
 
 # pa_dtype
-PA_F32, PA_I64, PA_I32, PA_U8, PA_F64 = 0, 1, 2, 3, 4
+PA_F32, PA_I64, PA_I32, PA_U8, PA_F64, PA_BF16, PA_F16 = 0, 1, 2, 3, 4, 5, 6
 
 _TORCH_TO_PA = {
     torch.float32: PA_F32,
@@ -195,6 +195,35 @@ class MlpDesc(C.Structure):
         ("batch_norm", C.c_int32),
         ("dropout", C.c_int32),
         ("residual", C.c_int32),
+    ]
+
+
+class RecurrenceArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32), ("dtype", C.c_int32), ("gate_dtype", C.c_int32),
+        ("gate_logits", C.c_int32), ("reverse", C.c_int32), ("D", C.c_int32),
+        ("B", C.c_int64), ("T", C.c_int64),
+        ("x", C.c_void_p), ("x_b", C.c_int64), ("x_t", C.c_int64),
+        ("gate", C.c_void_p), ("gate_b", C.c_int64), ("gate_t", C.c_int64),
+        ("h0", C.c_void_p),
+        ("resets", C.c_void_p), ("resets_b", C.c_int64), ("resets_t", C.c_int64),
+        ("lengths", C.c_void_p),
+        ("h", C.c_void_p), ("last", C.c_void_p), ("carries", C.c_void_p), ("scratch", C.c_void_p),
+        ("d_h", C.c_void_p), ("d_h_b", C.c_int64), ("d_h_t", C.c_int64), ("d_last", C.c_void_p),
+        ("d_x", C.c_void_p), ("d_gate", C.c_void_p), ("d_h0", C.c_void_p),
+    ]
+
+
+class LogProbsArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32), ("dtype", C.c_int32), ("action_dtype", C.c_int32), ("A", C.c_int32),
+        ("rows", C.c_int64),
+        ("logits", C.c_void_p), ("ld", C.c_int64), ("actions", C.c_void_p),
+        ("mask", C.c_void_p), ("ldm", C.c_int64),
+        ("temperature", C.c_float), ("top", C.c_int32),
+        ("log_prob", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p),
+        ("top_actions", C.c_void_p), ("top_log_probs", C.c_void_p), ("scratch", C.c_void_p),
+        ("d_log_prob", C.c_void_p), ("d_entropy", C.c_void_p), ("d_logits", C.c_void_p),
     ]
 
 
@@ -400,6 +429,18 @@ SIGNATURES = {
     "pa_sample_indices_rounds": (C.c_int, [C.c_int64, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32,
                                            _P, C.c_int32, _P]),
     "pa_gather_planes": (C.c_int, [_P, C.c_int64, C.c_int32, _P, C.c_int32, _P, _P]),
+    "pa_embed_tokens": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int64,
+                                  C.c_float, _P, C.c_int32, _P]),
+    "pa_embed_tokens_grad_scratch": (C.c_int64, [C.c_int64, C.c_int32]),
+    "pa_embed_tokens_grad": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, C.c_int64,
+                                       C.c_int32, _P, _P, C.c_int32, _P]),
+    "pa_gated_recurrence_scratch": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32]),
+    "pa_gated_recurrence_carries": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
+    "pa_gated_recurrence": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),
+    "pa_gated_recurrence_grad": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),
+    "pa_action_log_probs_scratch": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "pa_action_log_probs": (C.c_int, [C.POINTER(LogProbsArgs), _P]),
+    "pa_action_log_probs_grad": (C.c_int, [C.POINTER(LogProbsArgs), _P]),
     "pa_one_hot": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int32, _P, _P]),
     "pa_dqn_param_count": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "pa_dqn_param_offsets": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
