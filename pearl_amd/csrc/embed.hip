@@ -4,7 +4,7 @@
 //   out[i, :] = scale W[tok_i, :]          d_W[v, :] = scale sum_{i : tok_i = v} d_out[i, :]
 //
 // Both move rows and are bound by memory.  The gradient gathers instead of scattering: the tokens are
-// sorted, equal tokens are summed in index order in fp32 registers, each row of d_W is rounded and
+// grouped, equal tokens are summed in index order in fp32 registers, each row of d_W is rounded and
 // written once; no floating-point atomics, so equal inputs give equal bits.
 #include "seq_common.hpp"
 
@@ -62,29 +62,35 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs<T> a) {
 }
 
 // ---- gradient ------------------------------------------------------------------------------------
-// Sorting by counting: the place of token i among all is the number of tokens before it in the order
-// (token, index), counted against every other token from LDS.  n^2 comparisons need no passes, no
-// atomics and no further launches.  The launch also clears d_W: blocks behind the counting ones.
-constexpr int RANK_TILE = 4096;
+// Grouping equal tokens, in index order, in one launch and without a pass over the batch per digit:
+// workgroup w owns the tokens v with v mod W = w (neighbouring tokens, often alike in frequency, go to
+// different workgroups) and reads the whole list twice from L2.  First it counts its tokens, per wave
+// and token, and the tokens of the workgroups before it, which is where its part of the order begins;
+// then every wave walks its sixteenth of the list again and puts each token at its place.  A token that
+// fills the list costs one ballot per 64 entries like any other, so skew does not matter.  The blocks
+// behind clear d_W meanwhile.
+constexpr int BINS = 512;     // tokens per workgroup
+constexpr int GROUP_WAVES = 16;
 
-struct RankArgs {
+struct GroupArgs {
   const void* tokens; int64_t n;
   uint32_t vocab;
-  uint32_t* perm; uint32_t* keys;     // sorted: index and token of place p
-  int rank_blocks;
+  int owners, owner_shift;            // W, a power of two
+  uint32_t* perm; uint32_t* keys;     // grouped: index and token of place p
+  uint32_t* placed;                   // how many tokens have a row
   uint8_t* clear; int64_t clear_bytes;
 };
 
 template <typename I>
-__global__ __launch_bounds__(1024) void rank_kernel(RankArgs a) {
-  __shared__ __attribute__((aligned(16))) uint32_t tile[RANK_TILE];
-  __shared__ uint32_t counts[16][64];
+__global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
+  __shared__ uint32_t count[BINS * GROUP_WAVES];     // [token][wave]
+  __shared__ uint32_t wave_sum[GROUP_WAVES], wave_before[GROUP_WAVES], wave_all[GROUP_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if ((int)blockIdx.x >= a.rank_blocks) {
+  if ((int)blockIdx.x >= a.owners) {
     typedef uint32_t U __attribute__((ext_vector_type(4), aligned(2)));
     U zero = {0, 0, 0, 0};
-    const int64_t step = (int64_t)(gridDim.x - a.rank_blocks) * 1024 * 16;
-    for (int64_t o = ((int64_t)(blockIdx.x - a.rank_blocks) * 1024 + tid) * 16; o < a.clear_bytes; o += step) {
+    const int64_t step = (int64_t)(gridDim.x - a.owners) * 1024 * 16;
+    for (int64_t o = ((int64_t)(blockIdx.x - a.owners) * 1024 + tid) * 16; o < a.clear_bytes; o += step) {
       if (o + 16 <= a.clear_bytes)
         *reinterpret_cast<U*>(a.clear + o) = zero;
       else
@@ -93,73 +99,105 @@ __global__ __launch_bounds__(1024) void rank_kernel(RankArgs a) {
     return;
   }
   const I* tokens = reinterpret_cast<const I*>(a.tokens);
-  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
-  const uint32_t key = i < a.n ? token_key(tokens, i, a.vocab) : 0xffffffffu;
-  uint32_t before = 0;
-  for (int64_t base = 0; base < a.n; base += RANK_TILE) {
-    __syncthreads();
+  const uint32_t me = blockIdx.x, low = (uint32_t)a.owners - 1;
+  for (int k = tid; k < BINS * GROUP_WAVES; k += 1024) count[k] = 0;
+  __syncthreads();
+  // each wave's part of the list, in whole groups of 64
+  const int64_t part = (a.n + 64 * GROUP_WAVES - 1) / (64 * GROUP_WAVES) * 64;
+  const int64_t i0 = wave * part, i1 = i0 + part < a.n ? i0 + part : a.n;
+  uint32_t before = 0, all = 0;
+#pragma unroll 4
+  for (int64_t i = i0 + lane; i < i1; i += 64) {
+    const uint32_t key = token_key(tokens, i, a.vocab);
+    const bool valid = key < a.vocab;
+    before += valid && (key & low) < me;
+    all += valid;
+    if (valid && (key & low) == me) atomicAdd(&count[(key >> a.owner_shift) * GROUP_WAVES + wave], 1u);
+  }
 #pragma unroll
-    for (int k = tid; k < RANK_TILE; k += 1024)
-      tile[k] = base + k < a.n ? token_key(tokens, base + k, a.vocab) : 0xffffffffu;
-    __syncthreads();
-    // each wave counts a 16th of the tile, in groups of 64 that lie before, behind or at this block
-#pragma unroll 1
-    for (int g = wave * (RANK_TILE / 16 / 64); g < (wave + 1) * (RANK_TILE / 16 / 64); ++g) {
-      const int64_t group = base / 64 + g;
-      if (group * 64 >= a.n) break;
-      const uint4* q = reinterpret_cast<const uint4*>(tile + g * 64);
-      if (group < (int64_t)blockIdx.x) {
+  for (int o = 1; o < 64; o *= 2) {
+    before += __shfl_xor(before, o);
+    all += __shfl_xor(all, o);
+  }
+  if (lane == 0) {
+    wave_before[wave] = before;
+    wave_all[wave] = all;
+  }
+  __syncthreads();
+  // counts -> places: exclusive sums in the order (token, wave), from this workgroup's first place on
+  uint32_t sum = 0, c[GROUP_WAVES];
+  if (tid < BINS) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint4 t = q[k];
-          before += (t.x <= key) + (t.y <= key) + (t.z <= key) + (t.w <= key);
-        }
-      } else if (group > (int64_t)blockIdx.x) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint4 t = q[k];
-          before += (t.x < key) + (t.y < key) + (t.z < key) + (t.w < key);
-        }
-      } else {
-        for (int k = 0; k < 64; ++k) {
-          const uint32_t t = tile[g * 64 + k];
-          before += t < key || (t == key && k < lane);
-        }
-      }
+    for (int w = 0; w < GROUP_WAVES; ++w) {
+      c[w] = count[tid * GROUP_WAVES + w];
+      sum += c[w];
     }
   }
-  counts[wave][lane] = before;
-  __syncthreads();
-  if (wave == 0 && i < a.n) {
-    uint32_t place = 0;
+  uint32_t incl = sum;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) place += counts[w][lane];
-    a.perm[place] = (uint32_t)i;
-    a.keys[place] = key;
+  for (int o = 1; o < 64; o *= 2) {
+    const uint32_t y = __shfl_up(incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  uint32_t place = incl - sum, total = 0;
+  for (int w = 0; w < GROUP_WAVES; ++w) {
+    place += wave_before[w] + (w < wave ? wave_sum[w] : 0);
+    total += wave_all[w];
+  }
+  if (me == 0 && tid == 0) *a.placed = total;
+  if (tid < BINS) {
+#pragma unroll
+    for (int w = 0; w < GROUP_WAVES; ++w) {
+      count[tid * GROUP_WAVES + w] = place;
+      place += c[w];
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int64_t g = i0; g < i1; g += 64) {
+    const int64_t i = g + lane;
+    const uint32_t key = i < i1 ? token_key(tokens, i, a.vocab) : a.vocab;
+    uint64_t mine = __ballot(key < a.vocab && (key & low) == me);
+    while (mine) {
+      const int first = __ffsll((unsigned long long)mine) - 1;
+      const uint32_t k = __shfl(key, first);
+      const uint64_t same = __ballot(key == k);
+      uint32_t at = 0;          // this wave's own counter of the token
+      if (lane == first) at = atomicAdd(&count[(k >> a.owner_shift) * GROUP_WAVES + wave], (uint32_t)__popcll(same));
+      at = __shfl(at, first);
+      if (key == k) {
+        const uint32_t p = at + __popcll(same & ((1ull << lane) - 1));
+        a.perm[p] = (uint32_t)i;
+        a.keys[p] = k;
+      }
+      mine &= ~same;
+    }
   }
 }
 
-// The sorted places are cut into chunks of equal length, whatever the tokens: a token that is drawn
-// often is summed by many chunks.  A run of equal tokens that lies inside a chunk is rounded and
-// written there; the parts of one that passes a border go to `head` (it began before this chunk) and
-// `tail` (it began here and goes on), in fp32, and join_kernel adds them in order.
+// The places are cut into chunks of equal length, whatever the tokens: a token that is drawn often is
+// summed by many chunks, a few of which share a workgroup.  A run of equal tokens that lies inside a
+// chunk is rounded and written there.  The parts of one that passes a border are joined in order, in
+// fp32: inside a workgroup through LDS, between workgroups through `head` (a part that began before
+// this workgroup) and `tail` (one that began here and goes on) by join_kernel.
 template <typename T>
 struct SumArgs {
   const T* d_out; int64_t ldd;
   int dim;
   uint32_t vocab;
-  int64_t n, chunks;
-  int chunk;        // places per chunk
-  int lane_shift;   // log2 of the lanes that share a chunk
-  const uint32_t* perm; const uint32_t* keys;
-  float* head; float* tail;   // [chunks][dim]
+  int64_t groups;       // workgroups along the places
+  int chunk, subs;      // places per chunk, chunks per workgroup
+  int lane_shift;       // log2 of the lanes that share a chunk
+  const uint32_t* perm; const uint32_t* keys; const uint32_t* placed;
+  float* head; float* tail;   // [groups][dim]
   float scale;
   T* d_weight;
 };
 
 template <typename T, int V>
 __device__ __forceinline__ void write_row(const SumArgs<T>& a, uint32_t key, int c, const float (&acc)[V]) {
-  if (key >= a.vocab) return;
   float f[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) f[k] = acc[k] * a.scale;
@@ -177,65 +215,150 @@ __device__ __forceinline__ void write_partial(float* dst, int left, const float 
     if (k < left) dst[k] = acc[k];
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void sum_kernel(SumArgs<T> a) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int lanes = 1 << a.lane_shift;
-  const int64_t chunk = (int64_t)blockIdx.x * (256 >> a.lane_shift) + (threadIdx.x >> a.lane_shift);
-  const int c = (int)(blockIdx.y * 256 + (threadIdx.x & (lanes - 1))) * V;
-  if (chunk >= a.chunks || c >= a.dim) return;
-  const int left = a.dim - c;
-  const int64_t p0 = chunk * a.chunk;
-  const int64_t p1 = p0 + a.chunk < a.n ? p0 + a.chunk : a.n;
-  bool inside = p0 == 0 || a.keys[p0 - 1] != a.keys[p0];   // the run being summed began in this chunk
-  uint32_t run = a.keys[p0];
-  float acc[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-  for (int64_t p = p0; p < p1; ++p) {
-    const uint32_t key = a.keys[p];
-    const T* src = a.d_out + (int64_t)a.perm[p] * a.ldd + c;
-    const Pack<T, V> g = left >= V ? load_pack<T, V>(src) : load_part<T, V>(src, left);
-    if (key != run) {
-      if (inside) write_row<T, V>(a, run, c, acc);
-      else write_partial<V>(a.head + chunk * a.dim + c, left, acc);
-      inside = true;
-      run = key;
-#pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-    }
-    float f[V];
-    unpack<T, V>(g, f);
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] += f[k];
-  }
-  const bool goes_on = p1 < a.n && a.keys[p1] == run;
-  if (!inside) write_partial<V>(a.head + chunk * a.dim + c, left, acc);
-  else if (goes_on) write_partial<V>(a.tail + chunk * a.dim + c, left, acc);
-  else write_row<T, V>(a, run, c, acc);
-}
+constexpr int MAX_CHUNK = 32, MAX_SUBS = 64;
 
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(SumArgs<T> a) {
-  constexpr int V = 16 / (int)sizeof(T);
+__global__ __launch_bounds__(512) void sum_kernel(SumArgs<T> a) {
+  constexpr int V = 16 / (int)sizeof(T), AHEAD = 8;
+  extern __shared__ __attribute__((aligned(16))) float parts[];   // [2][threads][V]: heads, tails
+  __shared__ uint32_t keys[MAX_CHUNK * MAX_SUBS + 2], perm[MAX_CHUNK * MAX_SUBS];
+  const int lanes = 1 << a.lane_shift, threads = blockDim.x;
+  const int sub = threadIdx.x >> a.lane_shift, lane = threadIdx.x & (lanes - 1);
+  const int c = (int)(blockIdx.y * 256 + lane) * V;
+  const int left = a.dim - c;
+  const int64_t n = *a.placed;
+  const int span = a.subs * a.chunk;
+  const int64_t w0 = (int64_t)blockIdx.x * span;
+  if (w0 >= n) return;
+  const int here = (int)(w0 + span < n ? span : n - w0);
+  // keys[1 + k]: place w0 + k; one more at both ends, `vocab` where the list has none
+  for (int k = threadIdx.x; k < here + 2; k += threads) {
+    const int64_t p = w0 + k - 1;
+    keys[k] = p >= 0 && p < n ? a.keys[p] : a.vocab;
+    if (k < here) perm[k] = a.perm[w0 + k];
+  }
+  __syncthreads();
+  const int p0 = sub * a.chunk, p1 = p0 + a.chunk < here ? p0 + a.chunk : here;
+  if (p0 < p1 && left > 0) {
+    bool inside = keys[p0] != keys[p0 + 1];     // the run being summed began in this chunk
+    uint32_t run = keys[p0 + 1];
+    float acc[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+    for (int q = p0; q < p1; q += AHEAD) {
+      Pack<T, V> g[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (q + u >= p1) break;
+        const T* src = a.d_out + (int64_t)perm[q + u] * a.ldd + c;
+        g[u] = left >= V ? load_pack<T, V>(src) : load_part<T, V>(src, left);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (q + u >= p1) break;
+        const uint32_t key = keys[q + u + 1];
+        if (key != run) {
+          if (inside) write_row<T, V>(a, run, c, acc);
+          else
+#pragma unroll
+            for (int k = 0; k < V; ++k) parts[threadIdx.x * V + k] = acc[k];
+          inside = true;
+          run = key;
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+        }
+        float f[V];
+        unpack<T, V>(g[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += f[k];
+      }
+    }
+    if (inside && keys[p1 + 1] != run) write_row<T, V>(a, run, c, acc);
+    else
+#pragma unroll
+      for (int k = 0; k < V; ++k) parts[((inside ? threads : 0) + threadIdx.x) * V + k] = acc[k];
+  }
+  __syncthreads();
+  if (sub || left <= 0) return;
+  // the chunks' open ends, in order
+  float acc[V];
+  bool open = keys[0] == keys[1], began_here = false;   // a run is being joined; it began in this workgroup
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+  for (int s = 0; s < a.subs; ++s) {
+    const int b0 = s * a.chunk;
+    if (b0 >= here) break;
+    const int b1 = b0 + a.chunk < here ? b0 + a.chunk : here;
+    const uint32_t first = keys[b0 + 1], last = keys[b1];
+    if (keys[b0] == first) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += parts[((s << a.lane_shift) + lane) * V + k];
+      if (first != last || keys[b1 + 1] != last) {      // the run ends in this chunk
+        if (began_here) write_row<T, V>(a, first, c, acc);
+        else write_partial<V>(a.head + (int64_t)blockIdx.x * a.dim + c, left, acc);
+        open = false;
+      }
+    }
+    if (keys[b1 + 1] == last && (keys[b0] != first || first != last)) {   // one begins here and goes on
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] = parts[(threads + (s << a.lane_shift) + lane) * V + k];
+      open = began_here = true;
+    }
+  }
+  if (open) write_partial<V>((began_here ? a.tail : a.head) + (int64_t)blockIdx.x * a.dim + c, left, acc);
+}
+
+// One workgroup for each run that goes on behind the workgroup it began in: its tail, then the heads
+// of those it reaches, shared by the subgroups in contiguous parts.
+template <typename T>
+__global__ __launch_bounds__(512) void join_kernel(SumArgs<T> a) {
+  constexpr int V = 16 / (int)sizeof(T), AHEAD = 4;
+  extern __shared__ __attribute__((aligned(16))) float parts[];   // [threads][V]
+  const int64_t n = *a.placed;
+  const int64_t span = (int64_t)a.subs * a.chunk, w0 = blockIdx.x * span, w1 = w0 + span;
+  if (w1 >= n) return;
+  const uint32_t run = a.keys[w1 - 1];
+  if (a.keys[w1] != run) return;                                       // ends here
+  if (a.keys[w0] == run && w0 > 0 && a.keys[w0 - 1] == run) return;    // began before
   const int lanes = 1 << a.lane_shift;
-  const int64_t chunk = (int64_t)blockIdx.x * (256 >> a.lane_shift) + (threadIdx.x >> a.lane_shift);
-  const int c = (int)(blockIdx.y * 256 + (threadIdx.x & (lanes - 1))) * V;
-  if (chunk >= a.chunks || c >= a.dim) return;
-  const int64_t p0 = chunk * a.chunk, p1 = p0 + a.chunk;
-  if (p1 >= a.n) return;
-  const uint32_t run = a.keys[p1 - 1];
-  if (a.keys[p1] != run) return;                                        // ends here
-  if (a.keys[p0] == run && p0 > 0 && a.keys[p0 - 1] == run) return;     // began before this chunk
+  const int sub = threadIdx.x >> a.lane_shift, lane = threadIdx.x & (lanes - 1);
+  const int c = (int)(blockIdx.y * 256 + lane) * V;
   const int left = a.dim - c < V ? a.dim - c : V;
+  // how many of the next workgroups the run reaches, 64 at a time
+  int64_t reach = 0;
+  for (;;) {
+    const int64_t p = (blockIdx.x + 1 + reach + (threadIdx.x & 63)) * span;
+    const uint64_t other = __ballot(!(p < n && a.keys[p < n ? p : 0] == run));
+    if (other) {
+      reach += __ffsll((unsigned long long)other) - 1;
+      break;
+    }
+    reach += 64;
+  }
+  const int64_t share = (reach + a.subs - 1) / a.subs;
+  const int64_t h0 = blockIdx.x + 1 + sub * share;
+  const int64_t h1 = h0 + share < blockIdx.x + 1 + reach ? h0 + share : blockIdx.x + 1 + reach;
   float acc[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = k < left ? a.tail[chunk * a.dim + c + k] : 0.0f;
-  for (int64_t d = chunk + 1; d < a.chunks && a.keys[d * a.chunk] == run; ++d) {
+  for (int k = 0; k < V; ++k) acc[k] = sub == 0 && k < left ? a.tail[(int64_t)blockIdx.x * a.dim + c + k] : 0.0f;
+  for (int64_t h = h0; h < h1; h += AHEAD) {
+    float f[AHEAD][V];
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (k < left) acc[k] += a.head[d * a.dim + c + k];
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[u][k] = h + u < h1 && k < left ? a.head[(h + u) * a.dim + c + k] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += f[u][k];
   }
+#pragma unroll
+  for (int k = 0; k < V; ++k) parts[threadIdx.x * V + k] = acc[k];
+  __syncthreads();
+  if (sub || left <= 0) return;
+  for (int s = 1; s < a.subs && s * share < reach; ++s)
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += parts[((s << a.lane_shift) + lane) * V + k];
   write_row<T, V>(a, run, c, acc);
 }
 
@@ -245,27 +368,29 @@ int lane_shift_of(int dim, int v) {
   return s;
 }
 
-// places per chunk: enough chunks to fill the card, long enough that few runs pass a border
-int chunk_of(int64_t n) {
-  int c = 8;
-  while (c < 64 && n / c > 2048) c *= 2;
-  return c;
-}
-
 struct GradLayout {
-  int64_t perm, keys, head, tail, bytes;
-  int chunk;
-  int64_t chunks;
+  int64_t placed, perm, keys, head, tail, bytes;
+  int lane_shift, subs, chunk;
+  int64_t groups;
 };
-GradLayout grad_layout(int64_t n, int dim) {
+// Eight chunks per workgroup (narrow rows: more, for whole waves; wide ones: 512 threads), of a length that gives the card's
+// 256 CUs a workgroup each.
+GradLayout grad_layout(int64_t n, int dim, int dtype) {
   GradLayout l;
-  l.chunk = chunk_of(n);
-  l.chunks = ceil_div(n, l.chunk);
-  l.perm = 0;
-  l.keys = round_up(n * 4, 256);
+  const int v = 16 / elem_size(dtype);
+  l.lane_shift = lane_shift_of(dim, v);
+  l.subs = 8;
+  while ((l.subs << l.lane_shift) < 64) l.subs *= 2;
+  while ((l.subs << l.lane_shift) > 512) l.subs /= 2;
+  l.chunk = 2;
+  while (l.chunk < MAX_CHUNK && n > (int64_t)l.chunk * l.subs * 256) l.chunk *= 2;
+  l.groups = ceil_div(n, (int64_t)l.chunk * l.subs);
+  l.placed = 0;
+  l.perm = 256;
+  l.keys = l.perm + round_up(n * 4, 256);
   l.head = l.keys + round_up(n * 4, 256);
-  l.tail = l.head + round_up(l.chunks * dim * 4, 256);
-  l.bytes = l.tail + round_up(l.chunks * dim * 4, 256);
+  l.tail = l.head + round_up(l.groups * dim * 4, 256);
+  l.bytes = l.tail + round_up(l.groups * dim * 4, 256);
   return l;
 }
 
@@ -292,36 +417,42 @@ int embed_run(const void* weight, int64_t ldw, int64_t vocab, int32_t dim, const
 
 template <typename T>
 int grad_run(const void* d_out, int64_t ldd, const void* tokens, int32_t token_dtype, int64_t n,
-             float scale, int64_t vocab, int32_t dim, void* d_weight, uint8_t* scratch, hipStream_t s) {
+             float scale, int64_t vocab, int32_t dim, int32_t dtype, void* d_weight, uint8_t* scratch,
+             hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  const GradLayout l = grad_layout(n, dim);
-  RankArgs r;
+  const GradLayout l = grad_layout(n, dim, dtype);
+  GroupArgs r;
   r.tokens = tokens; r.n = n; r.vocab = (uint32_t)vocab;
+  r.owners = n ? 256 : 0; r.owner_shift = 8;
+  while (n && (int64_t)BINS << r.owner_shift < vocab) {
+    r.owners *= 2;
+    ++r.owner_shift;
+  }
   r.perm = reinterpret_cast<uint32_t*>(scratch + l.perm);
   r.keys = reinterpret_cast<uint32_t*>(scratch + l.keys);
-  r.rank_blocks = (int)ceil_div(n, 64);
+  r.placed = reinterpret_cast<uint32_t*>(scratch + l.placed);
   r.clear = reinterpret_cast<uint8_t*>(d_weight);
   r.clear_bytes = vocab * dim * (int64_t)sizeof(T);
   int64_t clear_blocks = ceil_div(r.clear_bytes, 1024 * 16 * 4);
   if (clear_blocks > 1024) clear_blocks = 1024;
-  const dim3 rank_grid((unsigned)(r.rank_blocks + clear_blocks));
-  if (token_dtype == PA_I64) hipLaunchKernelGGL((rank_kernel<int64_t>), rank_grid, dim3(1024), 0, s, r);
-  else hipLaunchKernelGGL((rank_kernel<int32_t>), rank_grid, dim3(1024), 0, s, r);
+  const dim3 group_grid((unsigned)(r.owners + clear_blocks));
+  if (token_dtype == PA_I64) hipLaunchKernelGGL((group_kernel<int64_t>), group_grid, dim3(1024), 0, s, r);
+  else hipLaunchKernelGGL((group_kernel<int32_t>), group_grid, dim3(1024), 0, s, r);
   PA_LAUNCH_CHECK();
   if (n == 0) return PA_OK;
   SumArgs<T> a;
   a.d_out = reinterpret_cast<const T*>(d_out); a.ldd = ldd; a.dim = dim; a.vocab = (uint32_t)vocab;
-  a.n = n; a.chunks = l.chunks; a.chunk = l.chunk;
-  a.lane_shift = lane_shift_of(dim, V);
-  a.perm = r.perm; a.keys = r.keys;
+  a.groups = l.groups; a.chunk = l.chunk; a.subs = l.subs; a.lane_shift = l.lane_shift;
+  a.perm = r.perm; a.keys = r.keys; a.placed = r.placed;
   a.head = reinterpret_cast<float*>(scratch + l.head);
   a.tail = reinterpret_cast<float*>(scratch + l.tail);
   a.scale = scale; a.d_weight = reinterpret_cast<T*>(d_weight);
-  const dim3 grid((unsigned)ceil_div(l.chunks, 256 >> a.lane_shift), (unsigned)ceil_div(dim, 256 * V));
-  hipLaunchKernelGGL((sum_kernel<T>), grid, dim3(256), 0, s, a);
+  const dim3 grid((unsigned)l.groups, (unsigned)ceil_div(dim, 256 * V));
+  const int threads = l.subs << l.lane_shift;
+  hipLaunchKernelGGL((sum_kernel<T>), grid, dim3(threads), 2 * threads * V * 4, s, a);
   PA_LAUNCH_CHECK();
-  if (l.chunks > 1) {
-    hipLaunchKernelGGL((join_kernel<T>), grid, dim3(256), 0, s, a);
+  if (l.groups > 1) {
+    hipLaunchKernelGGL((join_kernel<T>), grid, dim3(threads), threads * V * 4, s, a);
     PA_LAUNCH_CHECK();
   }
   return PA_OK;
@@ -347,8 +478,8 @@ extern "C" int pa_embed_tokens(const void* weight, int32_t dtype, int64_t ldw, i
   return embed_run<f16_t>(weight, ldw, vocab, dim, tokens, token_dtype, n, scale, out, s);
 }
 
-extern "C" int64_t pa_embed_tokens_grad_scratch(int64_t n, int32_t dim) {
-  return n <= 0 || dim <= 0 ? 0 : grad_layout(n, dim).bytes;
+extern "C" int64_t pa_embed_tokens_grad_scratch(int64_t n, int32_t dim, int32_t dtype) {
+  return n <= 0 || dim <= 0 || !elem_size(dtype) ? 0 : grad_layout(n, dim, dtype).bytes;
 }
 
 extern "C" int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ldd, const void* tokens,
@@ -357,7 +488,10 @@ extern "C" int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ld
   PA_REQUIRE(elem_size(dtype), PA_ERR_UNSUPPORTED, "pa_embed_tokens_grad: dtype %d", dtype);
   PA_REQUIRE(token_dtype == PA_I64 || token_dtype == PA_I32, PA_ERR_UNSUPPORTED,
              "pa_embed_tokens_grad: token dtype %d", token_dtype);
-  PA_REQUIRE(n >= 0 && n <= (1 << 20) && dim > 0 && vocab > 0 && vocab < 0xffffffffll, PA_ERR_INVALID,
+  // the grouping reads the token list once per 512 rows of the table
+  PA_REQUIRE(n <= (1 << 26) && vocab <= (1 << 26), PA_ERR_UNSUPPORTED,
+             "pa_embed_tokens_grad: %lld tokens, %lld rows (up to 2^26 of each)", (long long)n, (long long)vocab);
+  PA_REQUIRE(n >= 0 && dim > 0 && vocab > 0, PA_ERR_INVALID,
              "pa_embed_tokens_grad: bad shape (n %lld, vocab %lld, dim %d)", (long long)n, (long long)vocab, dim);
   PA_REQUIRE(d_weight && (n == 0 || (d_out && tokens && scratch && ldd >= 0)), PA_ERR_INVALID,
              "pa_embed_tokens_grad: null pointer");
@@ -365,8 +499,8 @@ extern "C" int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ld
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   uint8_t* w = reinterpret_cast<uint8_t*>(scratch);
   if (dtype == PA_F32)
-    return grad_run<float>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, d_weight, w, s);
+    return grad_run<float>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, dtype, d_weight, w, s);
   if (dtype == PA_BF16)
-    return grad_run<bf16_t>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, d_weight, w, s);
-  return grad_run<f16_t>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, d_weight, w, s);
+    return grad_run<bf16_t>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, dtype, d_weight, w, s);
+  return grad_run<f16_t>(d_out, ldd, tokens, token_dtype, n, scale, vocab, dim, dtype, d_weight, w, s);
 }

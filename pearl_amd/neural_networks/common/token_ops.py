@@ -96,7 +96,7 @@ def embed_tokens_grad(d_out: Tensor, tokens: Tensor, vocab: int, scale: float = 
     tokens = tokens.contiguous()
     lib = N.lib()
     d_weight = torch.empty(vocab, dim, dtype=d_out.dtype, device=d_out.device)
-    scratch = scratch_of(lib.pa_embed_tokens_grad_scratch(n, dim), d_out.device)
+    scratch = scratch_of(lib.pa_embed_tokens_grad_scratch(n, dim, code), d_out.device)
     N.check(lib.pa_embed_tokens_grad(rows.data_ptr(), code, rows.stride(0), tokens.data_ptr(), index, n, scale,
                                      vocab, dim, d_weight.data_ptr(), N.ptr(scratch), d_out.device.index,
                                      N.stream_ptr(d_out.device)))
