@@ -1108,7 +1108,7 @@ typedef struct pa_recurrence_args {
   void* d_gate;               /* [B][T][D]                                                  */
   float* d_h0;                /* [B][D]; NULL: not wanted                                   */
 } pa_recurrence_args;
-int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D, int32_t dtype);
+int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D);
 int64_t pa_gated_recurrence_carries(int64_t B, int64_t T, int32_t D);
 int pa_gated_recurrence(const pa_recurrence_args* args, void* stream);
 int pa_gated_recurrence_grad(const pa_recurrence_args* args, void* stream);

@@ -434,7 +434,7 @@ SIGNATURES = {
     "pa_embed_tokens_grad_scratch": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32]),
     "pa_embed_tokens_grad": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, C.c_int64,
                                        C.c_int32, _P, _P, C.c_int32, _P]),
-    "pa_gated_recurrence_scratch": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int32]),
+    "pa_gated_recurrence_scratch": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
     "pa_gated_recurrence_carries": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
     "pa_gated_recurrence": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),
     "pa_gated_recurrence_grad": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),

@@ -20,7 +20,7 @@
 //
 // Backward, with G_t = dh_t + c_t and c_{t-1} = a_t G_t (0 at a reset), c_T = d_last:
 //   decay:  dx = G, dg = G h_{t-1};   logit:  dx = (1 - a) G, dg = a (1 - a) G (h_{t-1} - x);
-//   d_h0 = c_0.  The forward pass keeps the fp32 state in front of every tile (1 / 256 of the steps);
+//   d_h0 = c_0.  The forward pass keeps the fp32 state in front of every 128th step;
 // the states inside a tile are computed again from it rather than read back rounded.
 #include "seq_common.hpp"
 
@@ -29,8 +29,20 @@ using namespace pa::seq;
 
 namespace {
 
-constexpr int CL = 8;        // lanes side by side in a row
-constexpr int TG = 64 / CL;  // groups of consecutive steps per wave
+// A kernel's shape: NW waves, CL lanes side by side in a row (so 64 / CL groups of steps per wave), L
+// consecutive steps per lane, V channels per lane.
+template <int NW_, int CL_, int L_, int V_>
+struct Shape {
+  static constexpr int NW = NW_, CL = CL_, L = L_, V = V_, TG = 64 / CL_, STEPS = NW_ * TG * L_, SLAB = CL_ * V_;
+};
+typedef Shape<1, 16, 8, 2> Short;          // histories of up to 32 steps
+typedef Shape<8, 16, 4, 2> Middle;         // of up to 128
+typedef Shape<16, 32, 8, 2> Long;          // longer ones, forwards
+typedef Shape<8, 32, 8, 2> LongGrad;       // longer ones, backwards
+constexpr int KEEP = Long::STEPS / LongGrad::STEPS;
+static_assert(Short::SLAB <= 64 && Middle::SLAB <= 64 && Long::SLAB <= 64 && LongGrad::SLAB == Long::SLAB,
+              "a lane of a wave carries the state of each channel");
+static_assert(Long::STEPS % LongGrad::STEPS == 0 && Long::NW % KEEP == 0, "states are kept in front of waves");
 
 template <typename T, typename G>
 struct RecArgs {
@@ -42,6 +54,7 @@ struct RecArgs {
   int64_t B, T_; int D;
   int reverse;
   int slabs, chunks; int64_t chunk_tiles, tiles;
+  int64_t kept;                                  // states kept per history: the gradient's tiles
   float* agg_a; float* agg_h; uint8_t* agg_r;    // [B][chunks][D], [B][chunks]: the chunks' pairs
   T* h; float* last; float* carries;             // [B][T][D], [B][D] or null, [B][tiles][D] or null
   const T* dh; int64_t dh_b, dh_t;               // or null: zeros
@@ -49,90 +62,206 @@ struct RecArgs {
   T* dx; G* dg; float* dh0;                      // dh0 or null
 };
 
-// a and 1 - a of a logit; both to a few ulp, also where one of them is tiny
-__device__ __forceinline__ void gate_of(float z, float& a, float& keep) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * fabsf(z));
-  const float hi = __builtin_amdgcn_rcpf(1.0f + e), lo = e * hi;
-  a = z >= 0.0f ? hi : lo;
-  keep = z >= 0.0f ? lo : hi;
-  if (z != z) a = keep = z;
+// a and 1 - a of a logit, both to a few ulp, also where one of them is tiny.  Below -80 a stays at 2e-35
+// (exp would overflow); NaN stays NaN (maximum, not fmax).
+__device__ __forceinline__ float exp_minus(float z) {
+  return __builtin_amdgcn_exp2f(-1.44269504088896340736f * __builtin_elementwise_maximum(z, -80.0f));
+}
+__device__ __forceinline__ void gate_of(float e, float& a, float& keep) {
+  a = __builtin_amdgcn_rcpf(1.0f + e);
+  keep = e * a;
 }
 
-template <typename T, typename G, int NW, int L>
+template <typename T, typename G, typename S>
 struct Tile {
-  static constexpr int V = 16 / (int)sizeof(T);   // channels per lane
-  static constexpr int STEPS = NW * TG * L;
-  static constexpr int SLAB = CL * V;
-  Pack<T, V> x[L];
-  Pack<G, V> g[L];
-  uint32_t resets;   // bit i: step i of this lane begins an episode
+  Pack<T, S::V> x[S::L];
+  Pack<G, S::V> g[S::L];
+  uint32_t resets[S::L / 4];   // a byte per step
 };
 
-// the place of step `s` of a history of n steps
-__device__ __forceinline__ int64_t place_of(int64_t s, int64_t n, int reverse) {
-  return reverse && s < n ? n - 1 - s : s;
+// The rows of one tile of a history of n steps.  Its step j lies in row first + j, or, read backwards,
+// in row first + here - 1 - j.  A tile behind the end gets one row that exists, for its loads.
+struct Rows {
+  int64_t first;
+  int here;        // steps of the tile that lie inside the history, at least 1
+  int valid;       // the same, or 0
+};
+template <typename S>
+__device__ __forceinline__ Rows rows_of(int64_t tile, int64_t n, int reverse) {
+  const int64_t valid = n - tile * S::STEPS;
+  Rows r;
+  r.valid = valid <= 0 ? 0 : valid < S::STEPS ? (int)valid : S::STEPS;
+  r.here = r.valid ? r.valid : 1;
+  r.first = r.valid ? reverse ? valid - r.here : tile * S::STEPS : 0;
+  return r;
 }
-
-template <typename T, int V, int L>
-__device__ __forceinline__ void load_rows(Pack<T, V> (&r)[L], const T* base, int64_t stride, int64_t s0,
-                                          int64_t n, int reverse, int left) {
+// byte offset of step j within the tile's rows; steps behind the end fall on the last row.  Row strides
+// are below 2^23 bytes, so one 24-bit multiply-add forms it and 31 bits hold it.
+__device__ __forceinline__ uint32_t row_offset(int j, const Rows& r, int reverse, uint32_t stride, uint32_t at) {
+  const int k = j < r.here ? j : r.here - 1;
+  return __umul24(reverse ? r.here - 1 - k : k, stride) + at;
+}
+// In a full tile a lane's i-th row is the same distance from its first in every lane: `lane_rows` is the
+// lane's part of its address, in rows, and step_row(i) the uniform part.  Accesses go through buffer
+// descriptors, which take the uniform part in a scalar register and the lane's as one 32-bit offset:
+// pointers would hold two vector registers and an addition for every row in flight.
+template <typename S>
+__device__ __forceinline__ int lane_rows(int j, int reverse) {
+  return reverse ? S::STEPS - S::L - j : j;
+}
+template <typename S>
+__device__ __forceinline__ int step_row(int i, int reverse) {
+  return reverse ? S::L - 1 - i : i;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, 0x7ffffff0, 0x00020000);
+}
+template <typename T, int V, bool TINY>
+__device__ __forceinline__ Pack<T, V> buffer_load(__amdgpu_buffer_rsrc_t b, uint32_t lane, uint32_t row) {
+  Pack<T, V> p;
+  if constexpr (TINY) {      // rows of one element
 #pragma unroll
-  for (int i = 0; i < L; ++i) {
-    const int64_t s = s0 + i;
-#pragma unroll
-    for (int k = 0; k < Pack<T, V>::WORDS; ++k) r[i].w[k] = 0;
-    if (s < n && left > 0) {
-      const T* p = base + place_of(s, n, reverse) * stride;
-      r[i] = left >= V ? load_pack<T, V>(p) : load_part<T, V>(p, left);
-    }
+    for (int k = 0; k < Pack<T, V>::WORDS; ++k) p.w[k] = 0;
+    p.w[0] = sizeof(T) == 4 ? __builtin_amdgcn_raw_buffer_load_b32(b, lane, row, 0)
+                            : __builtin_amdgcn_raw_buffer_load_b16(b, lane, row, 0);
+  } else if constexpr (Pack<T, V>::WORDS == 1) {
+    p.w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, lane, row, 0);
+  } else {
+    static_assert(Pack<T, V>::WORDS == 2, "two channels per lane");
+    const auto u = __builtin_amdgcn_raw_buffer_load_b64(b, lane, row, 0);
+    p.w[0] = u[0];
+    p.w[1] = u[1];
+  }
+  return p;
+}
+template <typename T, int V, bool TINY>
+__device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t b, uint32_t lane, uint32_t row, const Pack<T, V>& p) {
+  if constexpr (TINY) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(p.w[0], b, lane, row, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16((uint16_t)p.w[0], b, lane, row, 0);
+  } else if constexpr (Pack<T, V>::WORDS == 1) {
+    __builtin_amdgcn_raw_buffer_store_b32(p.w[0], b, lane, row, 0);
+  } else {
+    typedef uint32_t U __attribute__((ext_vector_type(2)));
+    U u;
+    u.x = p.w[0];
+    u.y = p.w[1];
+    __builtin_amdgcn_raw_buffer_store_b64(u, b, lane, row, 0);
   }
 }
 
-template <typename T, typename G, int L>
-__device__ __forceinline__ uint32_t load_resets(const RecArgs<T, G>& a, int64_t b, int64_t s0, int64_t n) {
-  uint32_t bits = 0;
-  if (a.resets) {
+// The L rows of this lane from step j of the tile on, `c` channels into the row.  No branches between
+// them, so that a tile's loads all go out at once; the selects on the step ignore what does not belong.
+template <typename S, typename T, bool TINY>
+__device__ __forceinline__ void load_rows(Pack<T, S::V> (&p)[S::L], const T* base, int64_t stride, int j, const Rows& r,
+                                          int reverse, int c) {
+  constexpr int V = S::V, L = S::L;
+  const uint32_t step = (uint32_t)(stride * sizeof(T)), at = (uint32_t)(c * sizeof(T));
+  const __amdgpu_buffer_rsrc_t rows = buffer_at(base + r.first * stride);
+  if (r.valid == S::STEPS) {
+    const uint32_t off = __umul24(lane_rows<S>(j, reverse), step) + at;
 #pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (s0 + i < n && a.resets[b * a.r_b + place_of(s0 + i, n, a.reverse) * a.r_t]) bits |= 1u << i;
+    for (int i = 0; i < L; ++i) p[i] = buffer_load<T, V, TINY>(rows, off, step * step_row<S>(i, reverse));
+  } else {
+#pragma unroll
+    for (int i = 0; i < L; ++i) p[i] = buffer_load<T, V, TINY>(rows, row_offset(j + i, r, reverse, step, at), 0);
+  }
+}
+
+// A byte for each of the lane's steps, in the order of the steps.
+template <typename S, typename T, typename G>
+__device__ __forceinline__ void load_resets(uint32_t (&p)[S::L / 4], const RecArgs<T, G>& a, int64_t b, int j,
+                                            const Rows& r) {
+  if (!a.resets) {
+#pragma unroll
+    for (int k = 0; k < S::L / 4; ++k) p[k] = 0;
+    return;
+  }
+  const uint8_t* first = a.resets + b * a.r_b + r.first * a.r_t;
+  if (r.valid == S::STEPS && a.r_t == 1) {
+    typedef uint32_t U __attribute__((aligned(1), may_alias));
+    const U* q = reinterpret_cast<const U*>(first + lane_rows<S>(j, a.reverse));
+#pragma unroll
+    for (int k = 0; k < S::L / 4; ++k) p[k] = q[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < S::L / 4; ++k) p[k] = 0;
+#pragma unroll
+    for (int i = 0; i < S::L; ++i) {
+      const uint32_t v = first[row_offset(j + i, r, a.reverse, (uint32_t)a.r_t, 0)];
+      const int at = r.valid == S::STEPS ? step_row<S>(i, a.reverse) : i;
+      const uint32_t byte = v && j + i < r.valid ? 1u << (8 * (at & 3)) : 0;
+#pragma unroll
+      for (int k = 0; k < S::L / 4; ++k) p[k] |= at / 4 == k ? byte : 0;
+    }
+  }
+}
+template <int W>
+__device__ __forceinline__ bool any_reset(const uint32_t (&p)[W]) {
+  uint32_t v = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) v |= p[k];
+  return v != 0;
+}
+// bit i: step i of this lane begins an episode.  In a full tile read backwards the bytes lie backwards.
+template <typename S>
+__device__ __forceinline__ uint32_t reset_bits(const uint32_t (&p)[S::L / 4], const Rows& r, int reverse) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < S::L; ++i) {
+    const int at = r.valid == S::STEPS ? step_row<S>(i, reverse) : i;
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < S::L / 4; ++k) w = at / 4 == k ? p[k] : w;
+    bits |= ((w >> (8 * (at & 3))) & 0xff ? 1u : 0u) << i;
   }
   return bits;
 }
 
-// the pair of one step: a = 1, b = 0 where the history has ended
-template <typename T, typename G, int V, bool LOGIT>
+// A lane's channels.  A row's last pack is moved back to end with the row, so every access is a whole
+// pack: the channels it shares with its neighbour are computed, and stored, by both alike.  Rows shorter
+// than a pack (TINY) are read element by element.
+template <int V, bool TINY>
+__device__ __forceinline__ int channel_of(int first, int D) {
+  return TINY ? first : first < D - V ? first : D - V;
+}
+
+// the factor and the input of one step; PLAIN: the step is known to lie inside the history
+template <typename T, typename G, int V, bool LOGIT, bool PLAIN>
 __device__ __forceinline__ void step_of(const Pack<T, V>& px, const Pack<G, V>& pg, bool on, float (&a)[V],
-                                        float (&keep)[V], float (&x)[V]) {
+                                        float (&keep)[V], float (&x)[V], float (&in)[V]) {
   unpack<T, V>(px, x);
   unpack<G, V>(pg, a);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     if constexpr (LOGIT) {
-      gate_of(a[v], a[v], keep[v]);
+      gate_of(exp_minus(a[v]), a[v], keep[v]);
+      in[v] = keep[v] * x[v];
     } else {
       keep[v] = 1.0f;
+      in[v] = x[v];
     }
-    if (!on) {
+    if (!PLAIN && !on) {
       a[v] = 1.0f;
-      keep[v] = 0.0f;
+      in[v] = 0.0f;
     }
   }
 }
 
-// (A, H, R) <- (A, H, R) o (pA, pH, pR)
-template <int V>
+// (A, H, R) <- (A, H, R) o (pA, pH, pR); PLAIN: no resets in this wave
+template <int V, bool PLAIN>
 __device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], bool& R, const float (&pA)[V],
                                         const float (&pH)[V], bool pR) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    H[v] = R ? H[v] : fmaf(A[v], pH[v], H[v]);
-    A[v] = R ? 0.0f : A[v] * pA[v];
+    H[v] = !PLAIN && R ? H[v] : fmaf(A[v], pH[v], H[v]);
+    A[v] = !PLAIN && R ? 0.0f : A[v] * pA[v];
   }
   R = R || pR;
 }
 
-// inclusive scan over the 8 groups of a wave, from the first (UP) or the last group on
-template <int V, bool UP>
+// inclusive scan over the groups of a wave, from the first (UP) or the last group on
+template <int V, int CL, bool UP, bool PLAIN>
 __device__ __forceinline__ void wave_scan(float (&A)[V], float (&H)[V], bool& R, int lane) {
 #pragma unroll
   for (int off = CL; off < 64; off *= 2) {
@@ -142,143 +271,244 @@ __device__ __forceinline__ void wave_scan(float (&A)[V], float (&H)[V], bool& R,
       pA[v] = UP ? __shfl_up(A[v], off) : __shfl_down(A[v], off);
       pH[v] = UP ? __shfl_up(H[v], off) : __shfl_down(H[v], off);
     }
-    const int pR = UP ? __shfl_up((int)R, off) : __shfl_down((int)R, off);
-    if (UP ? lane >= off : lane + off < 64) compose<V>(A, H, R, pA, pH, pR != 0);
+    const int pR = PLAIN ? 0 : UP ? __shfl_up((int)R, off) : __shfl_down((int)R, off);
+    if (UP ? lane >= off : lane + off < 64) compose<V, PLAIN>(A, H, R, pA, pH, pR != 0);
   }
 }
 
 // the state in front of this lane's steps: `in` (in front of the wave), then the groups before it
-template <int V, bool UP>
-__device__ __forceinline__ void state_in(float (&A)[V], float (&H)[V], bool R, const float* in, int lane,
+template <int V, int CL, bool UP, bool PLAIN>
+__device__ __forceinline__ void state_in(float (&A)[V], float (&H)[V], bool R, const float* front, int lane,
                                          float (&s)[V]) {
-  const int eR = UP ? __shfl_up((int)R, CL) : __shfl_down((int)R, CL);
+  float in[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) in[v] = front[v];
+  const int eR = PLAIN ? 0 : UP ? __shfl_up((int)R, CL) : __shfl_down((int)R, CL);
   const bool edge = UP ? lane < CL : lane >= 64 - CL;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float eA = UP ? __shfl_up(A[v], CL) : __shfl_down(A[v], CL);
     const float eH = UP ? __shfl_up(H[v], CL) : __shfl_down(H[v], CL);
-    s[v] = edge ? in[v] : eR ? eH : fmaf(eA, in[v], eH);
+    s[v] = edge ? in[v] : !PLAIN && eR ? eH : fmaf(eA, in[v], eH);
   }
 }
 
-template <typename T, typename G, int NW, int L>
-struct Shared {
-  static constexpr int SLAB = Tile<T, G, NW, L>::SLAB;
+// The waves' pairs of a tile and the states in front of the waves.
+template <int NW, int SLAB>
+struct Pairs {
   float A[NW][SLAB], H[NW][SLAB], in[NW][SLAB];
   int R[NW];
 };
+template <int V, int NW, int SLAB>
+__device__ __forceinline__ void put_pair(Pairs<NW, SLAB>& p, int wave, int slot, const float (&A)[V], const float (&H)[V],
+                                         bool R) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    p.A[wave][slot + v] = A[v];
+    p.H[wave][slot + v] = H[v];
+  }
+  p.R[wave] = R;
+}
+// One wave takes the states of the slab, one per lane, through the pairs of all waves; PROD also forms
+// the product.
+template <int NW, int SLAB, bool UP, bool PROD>
+__device__ __forceinline__ void join_waves(Pairs<NW, SLAB>& p, int lane, float& state, float& prod, bool& forgot) {
+  if (lane >= SLAB) return;
+  constexpr int AHEAD = NW < 4 ? NW : 4;      // pairs read at once: all of them would take 3 NW registers
+#pragma unroll 1
+  for (int k0 = 0; k0 < NW; k0 += AHEAD) {
+    float A[AHEAD], H[AHEAD];
+    int R[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int w = UP ? k0 + k : NW - 1 - k0 - k;
+      A[k] = p.A[w][lane];
+      H[k] = p.H[w][lane];
+      R[k] = p.R[w];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      p.in[UP ? k0 + k : NW - 1 - k0 - k][lane] = state;
+      const float next = fmaf(A[k], state, H[k]);
+      state = R[k] ? H[k] : next;
+      if constexpr (PROD) {
+        prod = R[k] ? 0.0f : prod * A[k];
+        forgot = forgot || R[k];
+      }
+    }
+  }
+}
+
+// The state in front of a chunk: the composition of the chunks before it (UP; behind it, down), scanned
+// like steps, one chunk per group of lanes.
+template <typename T, typename G, typename S, bool UP, bool TINY>
+__device__ __forceinline__ void through_chunks(const RecArgs<T, G>& a, Pairs<S::NW, S::SLAB>& pairs, int64_t b, int chunk,
+                                               int lane, int wave, int slot, int c, float& state) {
+  constexpr int V = S::V, GROUPS = S::NW * S::TG;
+  const int first = UP ? 0 : chunk + 1, last = UP ? chunk : a.chunks;     // [first, last)
+  for (int done = 0; done < last - first; done += GROUPS) {
+    const int g = wave * S::TG + lane / S::CL;
+    const int k = UP ? first + done + g : last - 1 - done - (GROUPS - 1 - g);
+    float A[V], H[V], prod = 0.0f;
+    bool R = false, forgot = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      A[v] = 1.0f;
+      H[v] = 0.0f;
+    }
+    if (k >= first && k < last) {
+      const int64_t o = b * a.chunks + k;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (!TINY || v < a.D) {
+          A[v] = a.agg_a[o * a.D + c + v];
+          H[v] = a.agg_h[o * a.D + c + v];
+        }
+      R = a.agg_r[o];
+    }
+    wave_scan<V, S::CL, UP, false>(A, H, R, lane);
+    if (UP ? lane >= 64 - S::CL : lane < S::CL) put_pair<V>(pairs, wave, slot, A, H, R);
+    __syncthreads();
+    if (wave == 0) join_waves<S::NW, S::SLAB, UP, false>(pairs, lane, state, prod, forgot);
+    __syncthreads();
+  }
+}
+
+// Store of one pack: of step j + i of a full tile, whose first row is `first`; and of step s of a history
+// of n steps, anywhere.
+template <typename S, typename T, bool TINY>
+__device__ __forceinline__ void put_row(T* first, int i, int j, int reverse, int c, int D, const Pack<T, S::V>& p) {
+  const uint32_t step = (uint32_t)(D * sizeof(T));
+  buffer_store<T, S::V, TINY>(buffer_at(first), __umul24(lane_rows<S>(j, reverse), step) + (uint32_t)(c * sizeof(T)),
+                              step * step_row<S>(i, reverse), p);
+}
+template <typename S, typename T, bool TINY>
+__device__ __forceinline__ void put_step(T* base, int64_t s, int64_t n, int reverse, int c, int D, const Pack<T, S::V>& p) {
+  T* row = base + (reverse && s < n ? n - 1 - s : s) * D + c;
+  if constexpr (!TINY) store_pack<T, S::V>(row, p);
+  else store_part<T, S::V>(row, p, D);
+}
+
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 
 // LOGIT gates or decay gates; EMIT: states out, else the pair of a chunk alone
-template <typename T, typename G, int NW, int L, bool LOGIT, bool EMIT>
-__global__ __launch_bounds__(NW * 64) void recurrence_kernel(RecArgs<T, G> a) {
-  using Ti = Tile<T, G, NW, L>;
-  constexpr int V = Ti::V, SLAB = Ti::SLAB;
-  __shared__ Shared<T, G, NW, L> sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <typename T, typename G, typename S, bool LOGIT, bool EMIT, bool TINY>
+__global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a) {
+  constexpr int V = S::V, SLAB = S::SLAB, NW = S::NW, CL = S::CL, L = S::L;
+  __shared__ Pairs<NW, SLAB> pairs;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs, chunk = blockIdx.x / a.slabs;
-  const int cl = (lane & (CL - 1)) * V;
-  const int c = slab * SLAB + cl;
-  const int left = a.D - c;
-  const int own = slab * SLAB + tid;                 // the channel whose state thread tid < SLAB carries
-  const bool owner = tid < SLAB && own < a.D;
+  const int slot = (lane & (CL - 1)) * V;
+  const bool active = slab * SLAB + slot < a.D;
+  const int c = active ? channel_of<V, TINY>(slab * SLAB + slot, a.D) : 0;
+  // lane k of wave 0 carries the state of this channel
+  const int own = channel_of<V, TINY>(slab * SLAB + lane / V * V, a.D) + lane % V;
+  const bool owner = wave == 0 && lane < SLAB && slab * SLAB + lane / V * V < a.D && own < a.D;
+  const int j = (wave * S::TG + lane / CL) * L;             // this lane's first step in a tile
   const int64_t tile0 = chunk * a.chunk_tiles;
   const int64_t tile1 = tile0 + a.chunk_tiles < a.tiles ? tile0 + a.chunk_tiles : a.tiles;
   for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y) {
     int64_t n = a.T_;
     if (a.lengths) {
-      n = a.lengths[b];
-      n = n < 0 ? 0 : n > a.T_ ? a.T_ : n;
+      const int64_t len = __builtin_amdgcn_readfirstlane(a.lengths[b]);
+      n = len < 0 ? 0 : len > n ? n : len;
     }
-    const T* xb = a.x + b * a.x_b + c;
-    const G* gb = a.g + b * a.g_b + c;
-    float state = 0.0f, prod = 1.0f;
+    const T* xb = a.x + b * a.x_b;
+    const G* gb = a.g + b * a.g_b;
+    Tile<T, G, S> cur;
+    Rows rows = rows_of<S>(tile0, n, a.reverse);
+    load_rows<S, T, TINY>(cur.x, xb, a.x_t, j, rows, a.reverse, c);
+    load_rows<S, G, TINY>(cur.g, gb, a.g_t, j, rows, a.reverse, c);
+    load_resets<S>(cur.resets, a, b, j, rows);
+    float state = EMIT && owner && a.h0 ? a.h0[b * a.D + own] : 0.0f, prod = 1.0f;
     bool forgot = false;
-    if (EMIT && owner) {
-      state = a.h0 ? a.h0[b * a.D + own] : 0.0f;
-      for (int k = 0; k < chunk; ++k) {
-        const int64_t o = b * a.chunks + k;
-        state = a.agg_r[o] ? a.agg_h[o * a.D + own] : fmaf(a.agg_a[o * a.D + own], state, a.agg_h[o * a.D + own]);
-      }
-    }
-    Ti cur;
-    int64_t s0 = tile0 * Ti::STEPS + (wave * TG + lane / CL) * L;
-    load_rows<T, V, L>(cur.x, xb, a.x_t, s0, n, a.reverse, left);
-    load_rows<G, V, L>(cur.g, gb, a.g_t, s0, n, a.reverse, left);
-    cur.resets = load_resets<T, G, L>(a, b, s0, n);
-    for (int64_t tile = tile0; tile < tile1; ++tile, s0 += Ti::STEPS) {
-      Ti next;
-      const int64_t s1 = s0 + Ti::STEPS;
-      const int64_t lim = tile + 1 < tile1 ? n : 0;   // nothing behind the last tile
-      load_rows<T, V, L>(next.x, xb, a.x_t, s1, lim ? n : 0, a.reverse, left);
-      load_rows<G, V, L>(next.g, gb, a.g_t, s1, lim ? n : 0, a.reverse, left);
-      next.resets = lim ? load_resets<T, G, L>(a, b, s1, n) : 0;
+    if (EMIT && chunk) through_chunks<T, G, S, true, TINY>(a, pairs, b, chunk, lane, wave, slot, c, state);
+    for (int64_t tile = tile0; tile < tile1; ++tile) {
+      Tile<T, G, S> next;
+      const Rows after = rows_of<S>(tile + 1 < tile1 ? tile + 1 : tile, n, a.reverse);
+      load_rows<S, T, TINY>(next.x, xb, a.x_t, j, after, a.reverse, c);
+      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
+      load_resets<S>(next.resets, a, b, j, after);
 
-      float A[L][V], H[L][V];
-      bool R = false;
+      // Most waves of most tiles have no reset and no step behind the end; without the selects for
+      // those a step costs half the instructions.
+      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets));
+      uint32_t resets = 0;
+      float A[L][V], H[L][V], sA[V], sH[V];
+      bool sR = false;
+      const auto scan = [&](auto is_plain) {
+        constexpr bool PLAIN = decltype(is_plain)::value;
 #pragma unroll
-      for (int i = 0; i < L; ++i) {
-        float f[V], keep[V], x[V];
-        step_of<T, G, V, LOGIT>(cur.x[i], cur.g[i], s0 + i < n, f, keep, x);
-        const bool r = (cur.resets >> i) & 1;
-        R = R || r;
+        for (int i = 0; i < L; ++i) {
+          float f[V], keep[V], x[V], in[V];
+          step_of<T, G, V, LOGIT, PLAIN>(cur.x[i], cur.g[i], j + i < rows.valid, f, keep, x, in);
+          const bool r = !PLAIN && ((resets >> i) & 1);
+          sR = sR || r;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            A[i][v] = r ? 0.0f : i ? f[v] * A[i ? i - 1 : 0][v] : f[v];
+            H[i][v] = (r || !i) ? in[v] : fmaf(f[v], H[i ? i - 1 : 0][v], in[v]);
+          }
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float in = s0 + i < n ? (LOGIT ? keep[v] * x[v] : x[v]) : 0.0f;
-          A[i][v] = r ? 0.0f : i ? f[v] * A[i ? i - 1 : 0][v] : f[v];
-          H[i][v] = (r || !i) ? in : fmaf(f[v], H[i ? i - 1 : 0][v], in);
+          sA[v] = A[L - 1][v];
+          sH[v] = H[L - 1][v];
         }
+        wave_scan<V, CL, true, PLAIN>(sA, sH, sR, lane);
+      };
+      if (plain) {
+        scan(Bool<true>());
+      } else {
+        resets = reset_bits<S>(cur.resets, rows, a.reverse);
+        scan(Bool<false>());
       }
-      float sA[V], sH[V];
-      bool sR = R;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        sA[v] = A[L - 1][v];
-        sH[v] = H[L - 1][v];
-      }
-      wave_scan<V, true>(sA, sH, sR, lane);
-      if (lane >= 64 - CL) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          sh.A[wave][cl + v] = sA[v];
-          sh.H[wave][cl + v] = sH[v];
-        }
-        if (lane == 63) sh.R[wave] = sR;
-      }
+      if (lane >= 64 - CL) put_pair<V>(pairs, wave, slot, sA, sH, sR);
       __syncthreads();
-      if (tid < SLAB) {
-        if (EMIT && a.carries && owner) a.carries[(b * a.tiles + tile) * a.D + own] = state;
+      if (wave == 0) {
+        join_waves<NW, SLAB, true, !EMIT>(pairs, lane, state, prod, forgot);
+        if (EMIT && a.carries && owner) {
+          // a state for each of the gradient's tiles, which are shorter: those in front of some waves
+          constexpr int PARTS = S::STEPS == Long::STEPS ? KEEP : 1;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          if (EMIT) sh.in[w][tid] = state;
-          const bool r = sh.R[w];
-          state = r ? sh.H[w][tid] : fmaf(sh.A[w][tid], state, sh.H[w][tid]);
-          prod = r ? 0.0f : prod * sh.A[w][tid];
-          forgot = forgot || r;
+          for (int q = 0; q < PARTS; ++q)
+            if (tile * PARTS + q < a.kept)
+              a.carries[(b * a.kept + tile * PARTS + q) * a.D + own] = pairs.in[q * (NW / PARTS)][lane];
         }
       }
       __syncthreads();
       if constexpr (EMIT) {
-        float in[V];
-        state_in<V, true>(sA, sH, sR, &sh.in[wave][cl], lane, in);
-        bool r = false;
+        const auto emit = [&](auto is_plain) {
+          constexpr bool PLAIN = decltype(is_plain)::value;
+          float s[V];
+          state_in<V, CL, true, PLAIN>(sA, sH, sR, &pairs.in[wave][slot], lane, s);
+          if (active) {
+            T* const base = a.h + b * a.T_ * a.D;
+            bool r = false;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-          r = r || ((cur.resets >> i) & 1);
-          float h[V];
+            for (int i = 0; i < L; ++i) {
+              r = !PLAIN && (r || ((resets >> i) & 1));
+              float h[V];
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            h[v] = r ? H[i][v] : fmaf(A[i][v], in[v], H[i][v]);
-            if (s0 + i >= n) h[v] = 0.0f;
+              for (int v = 0; v < V; ++v) {
+                h[v] = r ? H[i][v] : fmaf(A[i][v], s[v], H[i][v]);
+                if (!PLAIN && j + i >= rows.valid) h[v] = 0.0f;
+              }
+              const Pack<T, V> p = pack<T, V>(h);
+              const int64_t step = tile * S::STEPS + j + i;
+              if (PLAIN) put_row<S, T, TINY>(base + rows.first * a.D, i, j, a.reverse, c, a.D, p);
+              else if (step < a.T_) put_step<S, T, TINY>(base, step, n, a.reverse, c, a.D, p);
+            }
           }
-          if (s0 + i < a.T_ && left > 0) {
-            const Pack<T, V> p = pack<T, V>(h);
-            T* dst = a.h + (b * a.T_ + place_of(s0 + i, n, a.reverse)) * a.D + c;
-            if (left >= V) store_pack<T, V>(dst, p);
-            else store_part<T, V>(dst, p, left);
-          }
-        }
+        };
+        if (plain) emit(Bool<true>());
+        else emit(Bool<false>());
       }
       cur = next;
+      rows = after;
     }
     if (owner) {
       if constexpr (EMIT) {
@@ -287,7 +517,7 @@ __global__ __launch_bounds__(NW * 64) void recurrence_kernel(RecArgs<T, G> a) {
         const int64_t o = b * a.chunks + chunk;
         a.agg_a[o * a.D + own] = prod;
         a.agg_h[o * a.D + own] = state;
-        if (tid == 0) a.agg_r[o] = forgot;     // the same in every slab
+        if (lane == 0) a.agg_r[o] = forgot;     // the same in every slab
       }
     }
   }
@@ -309,13 +539,12 @@ __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
   Pack<G, V> pg;
   px = left >= V ? load_pack<T, V>(a.x + b * a.x_b + c) : load_part<T, V>(a.x + b * a.x_b + c, left);
   pg = left >= V ? load_pack<G, V>(a.g + b * a.g_b + c) : load_part<G, V>(a.g + b * a.g_b + c, left);
-  float f[V], keep[V], x[V], h[V], old[V];
-  step_of<T, G, V, LOGIT>(px, pg, true, f, keep, x);
+  float f[V], keep[V], x[V], in[V], h[V], old[V];
+  step_of<T, G, V, LOGIT, true>(px, pg, true, f, keep, x, in);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     old[v] = a.h0 && v < left ? a.h0[b * a.D + c + v] : 0.0f;
-    const float in = LOGIT ? keep[v] * x[v] : x[v];
-    h[v] = r ? in : fmaf(f[v], old[v], in);
+    h[v] = r ? in[v] : fmaf(f[v], old[v], in[v]);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -329,229 +558,234 @@ __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
 }
 
 // EMIT: gradients out; else the pair of a chunk's adjoint c_{t-1} = a_t (dh_t + c_t) alone.
-template <typename T, typename G, int NW, int L, bool LOGIT, bool EMIT>
-__global__ __launch_bounds__(NW * 64) void recurrence_grad_kernel(RecArgs<T, G> a) {
-  using Ti = Tile<T, G, NW, L>;
-  constexpr int V = Ti::V, SLAB = Ti::SLAB;
-  __shared__ Shared<T, G, NW, L> fw, bw;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <typename T, typename G, typename S, bool LOGIT, bool EMIT, bool TINY>
+__global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, G> a) {
+  constexpr int V = S::V, SLAB = S::SLAB, NW = S::NW, CL = S::CL, L = S::L;
+  __shared__ Pairs<NW, SLAB> fw, bw;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs;
   const int chunk = blockIdx.x / a.slabs + (EMIT ? 0 : 1);   // the first chunk's pair is not needed
-  const int cl = (lane & (CL - 1)) * V;
-  const int c = slab * SLAB + cl;
-  const int left = a.D - c;
-  // threads 0 .. SLAB-1 carry the adjoint of a channel; with more than one wave the next ones its state
-  const bool two = NW > 1;
-  const int own = slab * SLAB + (tid & (SLAB - 1));
-  const bool adjoint = tid < SLAB;
-  const bool stater = two ? tid >= 64 && tid < 64 + SLAB : tid < SLAB;
+  const int slot = (lane & (CL - 1)) * V;
+  const bool active = slab * SLAB + slot < a.D;
+  const int c = active ? channel_of<V, TINY>(slab * SLAB + slot, a.D) : 0;
+  // lane k of wave 0 carries the adjoint of this channel, lane k of the next wave (if there is one) its state
+  constexpr int STATE_WAVE = NW > 1 ? 1 : 0;
+  const int own = channel_of<V, TINY>(slab * SLAB + lane / V * V, a.D) + lane % V;
+  const bool owns = lane < SLAB && slab * SLAB + lane / V * V < a.D && own < a.D;
+  const bool owner = owns && wave == 0, stater = owns && wave == STATE_WAVE;
+  const int j = (wave * S::TG + lane / CL) * L;
   const int64_t tile0 = chunk * a.chunk_tiles;
   const int64_t tile1 = tile0 + a.chunk_tiles < a.tiles ? tile0 + a.chunk_tiles : a.tiles;
   for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y) {
     int64_t n = a.T_;
     if (a.lengths) {
-      n = a.lengths[b];
-      n = n < 0 ? 0 : n > a.T_ ? a.T_ : n;
+      const int64_t len = __builtin_amdgcn_readfirstlane(a.lengths[b]);
+      n = len < 0 ? 0 : len > n ? n : len;
     }
-    const T* xb = a.x + b * a.x_b + c;
-    const G* gb = a.g + b * a.g_b + c;
-    const T* db = a.dh ? a.dh + b * a.dh_b + c : nullptr;
-    float back = 0.0f, prod = 1.0f;
-    bool forgot = false;
-    if (EMIT && adjoint && own < a.D) {
-      back = a.d_last ? a.d_last[b * a.D + own] : 0.0f;
-      for (int k = a.chunks - 1; k > chunk; --k) {
-        const int64_t o = b * a.chunks + k;
-        back = a.agg_r[o] ? a.agg_h[o * a.D + own] : fmaf(a.agg_a[o * a.D + own], back, a.agg_h[o * a.D + own]);
-      }
-    }
-    Ti cur;
+    const T* xb = a.x + b * a.x_b;
+    const G* gb = a.g + b * a.g_b;
+    const T* db = a.dh ? a.dh + b * a.dh_b : xb;      // no gradient of h: any rows, then zeros
+    const int64_t d_t = a.dh ? a.dh_t : a.x_t;
+    Tile<T, G, S> cur;
     Pack<T, V> dcur[L];
-    int64_t s0 = (tile1 - 1) * Ti::STEPS + (wave * TG + lane / CL) * L;
-    if constexpr (EMIT) load_rows<T, V, L>(cur.x, xb, a.x_t, s0, n, a.reverse, left);
-    load_rows<G, V, L>(cur.g, gb, a.g_t, s0, n, a.reverse, left);
-    load_rows<T, V, L>(dcur, db, a.dh_t, s0, db ? n : 0, a.reverse, left);
-    cur.resets = load_resets<T, G, L>(a, b, s0, n);
-    for (int64_t tile = tile1 - 1; tile >= tile0; --tile, s0 -= Ti::STEPS) {
-      Ti next;
+    Rows rows = rows_of<S>(tile1 - 1, n, a.reverse);
+    if constexpr (EMIT) load_rows<S, T, TINY>(cur.x, xb, a.x_t, j, rows, a.reverse, c);
+    load_rows<S, G, TINY>(cur.g, gb, a.g_t, j, rows, a.reverse, c);
+    load_rows<S, T, TINY>(dcur, db, d_t, j, rows, a.reverse, c);
+    load_resets<S>(cur.resets, a, b, j, rows);
+    // the kept state in front of the tile
+    float carry = EMIT && stater ? a.carries[(b * a.tiles + tile1 - 1) * a.D + own] : 0.0f;
+    float back = EMIT && owner && a.d_last ? a.d_last[b * a.D + own] : 0.0f, prod = 1.0f;
+    bool forgot = false;
+    if (EMIT && chunk + 1 < a.chunks)
+      through_chunks<T, G, S, false, TINY>(a, bw, b, chunk, lane, wave, slot, c, back);
+    for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
+      Tile<T, G, S> next;
       Pack<T, V> dnext[L];
-      const int64_t s1 = s0 - Ti::STEPS;
-      const bool more = tile > tile0;
-      if constexpr (EMIT) load_rows<T, V, L>(next.x, xb, a.x_t, s1, more ? n : s1, a.reverse, left);
-      load_rows<G, V, L>(next.g, gb, a.g_t, s1, more ? n : s1, a.reverse, left);
-      load_rows<T, V, L>(dnext, db, a.dh_t, s1, more && db ? n : s1, a.reverse, left);
-      next.resets = more ? load_resets<T, G, L>(a, b, s1, n) : 0;
-      float state = 0.0f;
-      if (EMIT && stater && own < a.D) state = a.carries[(b * a.tiles + tile) * a.D + own];
-
-      // this lane's pairs: forwards (A, H) and the adjoint's (A, C)
-      float A[V], H[V], C[V];
-      bool R = false;
+      const int64_t tile_next = tile > tile0 ? tile - 1 : tile;
+      const Rows after = rows_of<S>(tile_next, n, a.reverse);
+      if constexpr (EMIT) load_rows<S, T, TINY>(next.x, xb, a.x_t, j, after, a.reverse, c);
+      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
+      load_rows<S, T, TINY>(dnext, db, d_t, j, after, a.reverse, c);
+      load_resets<S>(next.resets, a, b, j, after);
+      const float next_carry = EMIT && stater ? a.carries[(b * a.tiles + tile_next) * a.D + own] : 0.0f;
+      if (!a.dh) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        A[v] = 1.0f;
-        H[v] = C[v] = 0.0f;
+        for (int i = 0; i < L; ++i)
+#pragma unroll
+          for (int k = 0; k < Pack<T, V>::WORDS; ++k) dcur[i].w[k] = 0;
       }
-      float f[L][V], keep[L][V];
+      if constexpr (!EMIT) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) {
-        float x[V];
-        if constexpr (!EMIT) {
+        for (int i = 0; i < L; ++i)
 #pragma unroll
           for (int k = 0; k < Pack<T, V>::WORDS; ++k) cur.x[i].w[k] = 0;
-        }
-        const bool on = s0 + i < n;
-        step_of<T, G, V, LOGIT>(cur.x[i], cur.g[i], on, f[i], keep[i], x);
-        const bool r = (cur.resets >> i) & 1;
-        R = R || r;
+      }
+
+      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets));
+      uint32_t resets = 0;
+      float A[V], H[V], C[V], bA[V];     // this lane's pairs: forwards (A, H) and the adjoint's (bA, C)
+      float e[L][V];                     // exp(-gate), or the decay itself: half the registers of a and 1 - a
+      bool fR = false, bR = false;
+      // factor, 1 - factor and input of step i
+      const auto step = [&](auto is_plain, int i, float (&f)[V], float (&keep)[V], float (&x)[V], float (&in)[V]) {
+        constexpr bool PLAIN = decltype(is_plain)::value;
+        unpack<T, V>(cur.x[i], x);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float in = on ? (LOGIT ? keep[i][v] * x[v] : x[v]) : 0.0f;
-          H[v] = r ? in : fmaf(f[i][v], H[v], in);
-          A[v] = r ? 0.0f : A[v] * f[i][v];
-        }
-      }
-#pragma unroll
-      for (int i = L - 1; i >= 0; --i) {
-        float d[V];
-        unpack<T, V>(dcur[i], d);
-        const bool r = (cur.resets >> i) & 1;
-#pragma unroll
-        for (int v = 0; v < V; ++v) C[v] = r ? 0.0f : f[i][v] * (d[v] + C[v]);
-      }
-      float bA[V];
-      bool fR = R, bR = R;
-#pragma unroll
-      for (int v = 0; v < V; ++v) bA[v] = A[v];
-      wave_scan<V, false>(bA, C, bR, lane);
-      if (lane < CL) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          bw.A[wave][cl + v] = bA[v];
-          bw.H[wave][cl + v] = C[v];
-        }
-        if (lane == 0) bw.R[wave] = bR;
-      }
-      if constexpr (EMIT) {
-        wave_scan<V, true>(A, H, fR, lane);
-        if (lane >= 64 - CL) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            fw.A[wave][cl + v] = A[v];
-            fw.H[wave][cl + v] = H[v];
+          if constexpr (LOGIT) {
+            gate_of(e[i][v], f[v], keep[v]);
+            in[v] = keep[v] * x[v];
+          } else {
+            f[v] = e[i][v];
+            keep[v] = 1.0f;
+            in[v] = x[v];
           }
-          if (lane == 63) fw.R[wave] = fR;
+          if (!PLAIN && j + i >= rows.valid) {
+            f[v] = 1.0f;
+            in[v] = 0.0f;
+          }
         }
-      }
-      __syncthreads();
-      if (adjoint) {
+      };
+      const auto scan = [&](auto is_plain) {
+        constexpr bool PLAIN = decltype(is_plain)::value;
+        bool R = false;
 #pragma unroll
-        for (int w = NW - 1; w >= 0; --w) {
-          if (EMIT) bw.in[w][tid] = back;
-          const bool r = bw.R[w];
-          back = r ? bw.H[w][tid] : fmaf(bw.A[w][tid], back, bw.H[w][tid]);
-          prod = r ? 0.0f : prod * bw.A[w][tid];
-          forgot = forgot || r;
+        for (int v = 0; v < V; ++v) {
+          A[v] = 1.0f;
+          H[v] = C[v] = 0.0f;
         }
-      }
-      if (EMIT && stater) {
-        const int ch = tid & (SLAB - 1);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          fw.in[w][ch] = state;
-          state = fw.R[w] ? fw.H[w][ch] : fmaf(fw.A[w][ch], state, fw.H[w][ch]);
-        }
-      }
-      __syncthreads();
-      if constexpr (EMIT) {
-        float before[L][V], s[V], bk[V];
-        state_in<V, true>(A, H, fR, &fw.in[wave][cl], lane, s);
-        state_in<V, false>(bA, C, bR, &bw.in[wave][cl], lane, bk);
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-          float x[V];
-          unpack<T, V>(cur.x[i], x);
-          const bool r = (cur.resets >> i) & 1;
+          float f[V], keep[V], x[V], in[V], d[V];
+          unpack<G, V>(cur.g[i], e[i]);
+          if constexpr (LOGIT)
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            before[i][v] = r ? 0.0f : s[v];
-            const float in = s0 + i < n ? (LOGIT ? keep[i][v] * x[v] : x[v]) : 0.0f;
-            s[v] = r ? in : fmaf(f[i][v], s[v], in);
-          }
-        }
-#pragma unroll
-        for (int i = L - 1; i >= 0; --i) {
-          float x[V], d[V], dx[V], dg[V];
-          unpack<T, V>(cur.x[i], x);
+            for (int v = 0; v < V; ++v) e[i][v] = exp_minus(e[i][v]);
+          step(is_plain, i, f, keep, x, in);
           unpack<T, V>(dcur[i], d);
-          const bool r = (cur.resets >> i) & 1;
+          const bool r = !PLAIN && ((resets >> i) & 1);
+          R = R || r;
+          // the adjoint in front of these steps: each one's own gradient times the factors up to it
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float grad = d[v] + bk[v];
-            if constexpr (LOGIT) {
-              dx[v] = keep[i][v] * grad;
-              dg[v] = f[i][v] * dx[v] * (before[i][v] - x[v]);
-            } else {
-              dx[v] = grad;
-              dg[v] = grad * before[i][v];
-            }
-            if (s0 + i >= n) dx[v] = dg[v] = 0.0f;
-            bk[v] = r ? 0.0f : f[i][v] * grad;
-          }
-          if (s0 + i < a.T_ && left > 0) {
-            const int64_t o = (b * a.T_ + place_of(s0 + i, n, a.reverse)) * a.D + c;
-            const Pack<T, V> px = pack<T, V>(dx);
-            const Pack<G, V> pg = pack<G, V>(dg);
-            if (left >= V) {
-              store_pack<T, V>(a.dx + o, px);
-              store_pack<G, V>(a.dg + o, pg);
-            } else {
-              store_part<T, V>(a.dx + o, px, left);
-              store_part<G, V>(a.dg + o, pg, left);
-            }
+            if (!PLAIN && j + i >= rows.valid) d[v] = 0.0f;
+            H[v] = r ? in[v] : fmaf(f[v], H[v], in[v]);
+            A[v] = r ? 0.0f : A[v] * f[v];
+            C[v] = !PLAIN && R ? C[v] : fmaf(A[v], d[v], C[v]);
           }
         }
+        fR = bR = R;
+#pragma unroll
+        for (int v = 0; v < V; ++v) bA[v] = A[v];
+        wave_scan<V, CL, false, PLAIN>(bA, C, bR, lane);
+        if constexpr (EMIT) wave_scan<V, CL, true, PLAIN>(A, H, fR, lane);
+      };
+      if (plain) {
+        scan(Bool<true>());
+      } else {
+        resets = reset_bits<S>(cur.resets, rows, a.reverse);
+        scan(Bool<false>());
+      }
+      if (lane < CL) put_pair<V>(bw, wave, slot, bA, C, bR);
+      if (EMIT && lane >= 64 - CL) put_pair<V>(fw, wave, slot, A, H, fR);
+      __syncthreads();
+      if (wave == 0) join_waves<NW, SLAB, false, !EMIT>(bw, lane, back, prod, forgot);
+      if (EMIT && wave == STATE_WAVE) join_waves<NW, SLAB, true, false>(fw, lane, carry, prod, forgot);
+      __syncthreads();
+      if constexpr (EMIT) {
+        const auto emit = [&](auto is_plain) {
+          constexpr bool PLAIN = decltype(is_plain)::value;
+          float before[L][V], s[V], bk[V];
+          state_in<V, CL, true, PLAIN>(A, H, fR, &fw.in[wave][slot], lane, s);
+          state_in<V, CL, false, PLAIN>(bA, C, bR, &bw.in[wave][slot], lane, bk);
+          if (active) {
+            const int64_t base = b * a.T_ * a.D;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+              float f[V], keep[V], x[V], in[V];
+              step(is_plain, i, f, keep, x, in);
+              const bool r = !PLAIN && ((resets >> i) & 1);
+#pragma unroll
+              for (int v = 0; v < V; ++v) {
+                before[i][v] = r ? 0.0f : s[v];
+                s[v] = r ? in[v] : fmaf(f[v], s[v], in[v]);
+              }
+            }
+#pragma unroll
+            for (int i = L - 1; i >= 0; --i) {
+              float f[V], keep[V], x[V], in[V], d[V], dx[V], dg[V];
+              step(is_plain, i, f, keep, x, in);
+              unpack<T, V>(dcur[i], d);
+              const bool r = !PLAIN && ((resets >> i) & 1);
+#pragma unroll
+              for (int v = 0; v < V; ++v) {
+                if (!PLAIN && j + i >= rows.valid) d[v] = 0.0f;
+                const float grad = d[v] + bk[v];
+                if constexpr (LOGIT) {
+                  dx[v] = keep[v] * grad;
+                  dg[v] = f[v] * dx[v] * (before[i][v] - x[v]);
+                } else {
+                  dx[v] = grad;
+                  dg[v] = grad * before[i][v];
+                }
+                if (!PLAIN && j + i >= rows.valid) dx[v] = dg[v] = 0.0f;
+                bk[v] = r ? 0.0f : f[v] * grad;
+              }
+              const Pack<T, V> px = pack<T, V>(dx);
+              const Pack<G, V> pg = pack<G, V>(dg);
+              const int64_t s_i = tile * S::STEPS + j + i;
+              if (PLAIN) {
+                put_row<S, T, TINY>(a.dx + base + rows.first * a.D, i, j, a.reverse, c, a.D, px);
+                put_row<S, G, TINY>(a.dg + base + rows.first * a.D, i, j, a.reverse, c, a.D, pg);
+              } else if (s_i < a.T_) {
+                put_step<S, T, TINY>(a.dx + base, s_i, n, a.reverse, c, a.D, px);
+                put_step<S, G, TINY>(a.dg + base, s_i, n, a.reverse, c, a.D, pg);
+              }
+            }
+          }
+        };
+        if (plain) emit(Bool<true>());
+        else emit(Bool<false>());
       }
       cur = next;
+      rows = after;
+      carry = next_carry;
 #pragma unroll
       for (int i = 0; i < L; ++i) dcur[i] = dnext[i];
     }
-    if (adjoint && own < a.D) {
+    if (owner) {
       if constexpr (EMIT) {
         if (a.dh0 && chunk == 0) a.dh0[b * a.D + own] = back;
       } else {
         const int64_t o = b * a.chunks + chunk;
         a.agg_a[o * a.D + own] = prod;
         a.agg_h[o * a.D + own] = back;
-        if (tid == 0) a.agg_r[o] = forgot;
+        if (lane == 0) a.agg_r[o] = forgot;
       }
     }
   }
 }
-
-// Steps per tile: the forward and the backward pass agree on it, the kept states lie between tiles.
-// Histories of up to 32 steps take one wave per slab, longer ones eight.
-constexpr int SHORT = TG * 4;
-int64_t tile_steps(int64_t T) { return T <= SHORT ? SHORT : 8 * TG * 4; }
 
 struct Split {
   int slabs, chunks;
   int64_t tiles, chunk_tiles;
   int64_t agg_a, agg_h, agg_r, bytes;   // scratch layout
 };
-Split split_of(int64_t B, int64_t T, int D, int dtype) {
+// Fewer workgroups than CUs: the steps are cut, so that there are as many workgroups as CUs (one of 16
+// waves fills a CU's registers).  The pass over the chunks' pairs is another launch and the latency of a
+// tile: up to three tiles are walked as they are (7 x 1001 x 257 fp16, four tiles, odd rows: forwards
+// 29 us in one piece, 23 us in four).
+Split split_of(int64_t B, int64_t T, int D, bool grad) {
   Split s;
-  const int slab = CL * 16 / elem_size(dtype);
-  s.slabs = (int)ceil_div(D, slab);
-  s.tiles = ceil_div(T, tile_steps(T));
+  const bool brief = T <= Short::STEPS, middle = T <= Middle::STEPS;
+  s.slabs = (int)ceil_div(D, brief ? Short::SLAB : middle ? Middle::SLAB : Long::SLAB);
+  s.tiles = ceil_div(T, brief ? Short::STEPS : middle ? Middle::STEPS : grad ? LongGrad::STEPS : Long::STEPS);
   const int64_t groups = B * s.slabs;
-  int64_t chunks = groups >= 192 ? 1 : ceil_div(512, groups);
+  int64_t chunks = groups >= 192 || s.tiles <= 3 ? 1 : ceil_div(256, groups);
   if (chunks > s.tiles) chunks = s.tiles;
-  if (chunks > 128) chunks = 128;
-  if (chunks < 1) chunks = 1;
   s.chunk_tiles = ceil_div(s.tiles, chunks);
   s.chunks = (int)ceil_div(s.tiles, s.chunk_tiles);
-  if (s.chunks < 1) s.chunks = 1;
   const int64_t pairs = s.chunks > 1 ? B * s.chunks * D * 4 : 0;
   s.agg_a = 0;
   s.agg_h = round_up(pairs, 256);
@@ -560,8 +794,8 @@ Split split_of(int64_t B, int64_t T, int D, int dtype) {
   return s;
 }
 
-template <typename T, typename G, bool LOGIT>
-int run_forward(const pa_recurrence_args* p, const RecArgs<T, G>& a, hipStream_t s) {
+template <typename T, typename G, bool LOGIT, bool TINY>
+int run_forward(const RecArgs<T, G>& a, hipStream_t s) {
   if (a.T_ == 1 && !a.carries) {
     constexpr int V = 16 / (int)sizeof(T);
     hipLaunchKernelGGL((step_kernel<T, G, LOGIT>), dim3((unsigned)ceil_div(a.B * ceil_div(a.D, V), 256)),
@@ -570,49 +804,64 @@ int run_forward(const pa_recurrence_args* p, const RecArgs<T, G>& a, hipStream_t
     return PA_OK;
   }
   const unsigned rows = (unsigned)(a.B < 65535 ? a.B : 65535);
-  if (a.T_ <= SHORT) {
-    hipLaunchKernelGGL((recurrence_kernel<T, G, 1, 4, LOGIT, true>), dim3(a.slabs, rows), dim3(64), 0, s, a);
+  if (a.T_ <= Short::STEPS) {
+    hipLaunchKernelGGL((recurrence_kernel<T, G, Short, LOGIT, true, TINY>), dim3(a.slabs, rows),
+                       dim3(Short::NW * 64), 0, s, a);
+  } else if (a.T_ <= Middle::STEPS) {
+    hipLaunchKernelGGL((recurrence_kernel<T, G, Middle, LOGIT, true, TINY>), dim3(a.slabs, rows),
+                       dim3(Middle::NW * 64), 0, s, a);
   } else {
     if (a.chunks > 1) {
-      hipLaunchKernelGGL((recurrence_kernel<T, G, 8, 4, LOGIT, false>), dim3(a.slabs * (a.chunks - 1), rows),
-                         dim3(512), 0, s, a);
+      hipLaunchKernelGGL((recurrence_kernel<T, G, Long, LOGIT, false, TINY>),
+                         dim3(a.slabs * (a.chunks - 1), rows), dim3(Long::NW * 64), 0, s, a);
       PA_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL((recurrence_kernel<T, G, 8, 4, LOGIT, true>), dim3(a.slabs * a.chunks, rows), dim3(512),
-                       0, s, a);
+    hipLaunchKernelGGL((recurrence_kernel<T, G, Long, LOGIT, true, TINY>), dim3(a.slabs * a.chunks, rows),
+                       dim3(Long::NW * 64), 0, s, a);
+  }
+  PA_LAUNCH_CHECK();
+  return PA_OK;
+}
+
+template <typename T, typename G, bool LOGIT, bool TINY>
+int run_backward(const RecArgs<T, G>& a, hipStream_t s) {
+  const unsigned rows = (unsigned)(a.B < 65535 ? a.B : 65535);
+  if (a.T_ <= Short::STEPS) {
+    hipLaunchKernelGGL((recurrence_grad_kernel<T, G, Short, LOGIT, true, TINY>), dim3(a.slabs, rows),
+                       dim3(Short::NW * 64), 0, s, a);
+  } else if (a.T_ <= Middle::STEPS) {
+    hipLaunchKernelGGL((recurrence_grad_kernel<T, G, Middle, LOGIT, true, TINY>), dim3(a.slabs, rows),
+                       dim3(Middle::NW * 64), 0, s, a);
+  } else {
+    if (a.chunks > 1) {
+      hipLaunchKernelGGL((recurrence_grad_kernel<T, G, LongGrad, LOGIT, false, TINY>),
+                         dim3(a.slabs * (a.chunks - 1), rows), dim3(LongGrad::NW * 64), 0, s, a);
+      PA_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL((recurrence_grad_kernel<T, G, LongGrad, LOGIT, true, TINY>), dim3(a.slabs * a.chunks, rows),
+                       dim3(LongGrad::NW * 64), 0, s, a);
   }
   PA_LAUNCH_CHECK();
   return PA_OK;
 }
 
 template <typename T, typename G, bool LOGIT>
-int run_backward(const RecArgs<T, G>& a, hipStream_t s) {
-  const unsigned rows = (unsigned)(a.B < 65535 ? a.B : 65535);
-  if (a.T_ <= SHORT) {
-    hipLaunchKernelGGL((recurrence_grad_kernel<T, G, 1, 4, LOGIT, true>), dim3(a.slabs, rows), dim3(64), 0, s, a);
-  } else {
-    if (a.chunks > 1) {
-      hipLaunchKernelGGL((recurrence_grad_kernel<T, G, 8, 4, LOGIT, false>), dim3(a.slabs * (a.chunks - 1), rows),
-                         dim3(512), 0, s, a);
-      PA_LAUNCH_CHECK();
-    }
-    hipLaunchKernelGGL((recurrence_grad_kernel<T, G, 8, 4, LOGIT, true>), dim3(a.slabs * a.chunks, rows),
-                       dim3(512), 0, s, a);
-  }
-  PA_LAUNCH_CHECK();
-  return PA_OK;
+int run_either(const RecArgs<T, G>& a, bool grad, hipStream_t s) {
+  if (a.D < Short::V)
+    return grad ? run_backward<T, G, LOGIT, true>(a, s) : run_forward<T, G, LOGIT, true>(a, s);
+  return grad ? run_backward<T, G, LOGIT, false>(a, s) : run_forward<T, G, LOGIT, false>(a, s);
 }
 
 template <typename T, typename G>
 int run(const pa_recurrence_args* p, bool grad, hipStream_t s) {
-  const Split sp = split_of(p->B, p->T, p->D, p->dtype);
+  const Split sp = split_of(p->B, p->T, p->D, grad);
   uint8_t* scratch = reinterpret_cast<uint8_t*>(p->scratch);
   RecArgs<T, G> a;
   a.x = reinterpret_cast<const T*>(p->x); a.x_b = p->x_b; a.x_t = p->x_t;
   a.g = reinterpret_cast<const G*>(p->gate); a.g_b = p->gate_b; a.g_t = p->gate_t;
   a.h0 = p->h0; a.resets = p->resets; a.r_b = p->resets_b; a.r_t = p->resets_t;
   a.lengths = p->lengths; a.B = p->B; a.T_ = p->T; a.D = p->D; a.reverse = p->reverse;
-  a.slabs = sp.slabs; a.chunks = sp.chunks; a.chunk_tiles = sp.chunk_tiles; a.tiles = sp.tiles;
+  a.slabs = sp.slabs; a.chunks = sp.chunks; a.chunk_tiles = sp.chunk_tiles; a.tiles = sp.tiles; a.kept = split_of(p->B, p->T, p->D, true).tiles;
   a.agg_a = reinterpret_cast<float*>(scratch + sp.agg_a);
   a.agg_h = reinterpret_cast<float*>(scratch + sp.agg_h);
   a.agg_r = scratch + sp.agg_r;
@@ -620,9 +869,7 @@ int run(const pa_recurrence_args* p, bool grad, hipStream_t s) {
   a.dh = reinterpret_cast<const T*>(p->d_h); a.dh_b = p->d_h_b; a.dh_t = p->d_h_t;
   a.d_last = p->d_last;
   a.dx = reinterpret_cast<T*>(p->d_x); a.dg = reinterpret_cast<G*>(p->d_gate); a.dh0 = p->d_h0;
-  if (grad)
-    return p->gate_logits ? run_backward<T, G, true>(a, s) : run_backward<T, G, false>(a, s);
-  return p->gate_logits ? run_forward<T, G, true>(p, a, s) : run_forward<T, G, false>(p, a, s);
+  return p->gate_logits ? run_either<T, G, true>(a, grad, s) : run_either<T, G, false>(a, grad, s);
 }
 
 int dispatch(const pa_recurrence_args* p, bool grad, hipStream_t s) {
@@ -632,31 +879,37 @@ int dispatch(const pa_recurrence_args* p, bool grad, hipStream_t s) {
   return p->gate_dtype == PA_F32 ? run<f16_t, float>(p, grad, s) : run<f16_t, f16_t>(p, grad, s);
 }
 
-int check_args(const char* who, const pa_recurrence_args* p) {
+int check_args(const char* who, const pa_recurrence_args* p, bool grad) {
   PA_REQUIRE(p, PA_ERR_INVALID, "%s: null argument", who);
   PA_REQUIRE(elem_size(p->dtype), PA_ERR_UNSUPPORTED, "%s: input dtype %d", who, p->dtype);
   PA_REQUIRE(p->gate_dtype == p->dtype || p->gate_dtype == PA_F32, PA_ERR_UNSUPPORTED,
              "%s: gate dtype %d with input dtype %d (the input's own, or float32)", who, p->gate_dtype, p->dtype);
-  PA_REQUIRE(p->B >= 0 && p->T >= 1 && p->D >= 1 && p->D <= (1 << 24) && p->B <= (1ll << 31) / p->D, PA_ERR_INVALID,
+  const int64_t size = elem_size(p->dtype), gate_size = elem_size(p->gate_dtype), wide = 1 << 23;
+  const auto fits = [&](int64_t stride, int64_t bytes) { return stride >= 0 && stride * bytes < wide; };
+  PA_REQUIRE(fits(p->D, 4) && fits(p->x_t, size) && fits(p->gate_t, gate_size) && fits(p->resets_t, 1) &&
+                 fits(p->d_h_t, size), PA_ERR_UNSUPPORTED, "%s: a step is 2^23 bytes or more from the next", who);
+  PA_REQUIRE(p->B >= 0 && p->T >= 1 && p->D >= 1 && p->B <= (1ll << 31) / p->D, PA_ERR_INVALID,
              "%s: bad shape (batch %lld, time %lld, channels %d)", who, (long long)p->B, (long long)p->T, p->D);
   PA_REQUIRE(p->B == 0 || (p->x && p->gate), PA_ERR_INVALID, "%s: null pointer", who);
-  PA_REQUIRE(p->B == 0 || p->scratch || split_of(p->B, p->T, p->D, p->dtype).bytes == 0, PA_ERR_INVALID,
+  PA_REQUIRE(p->B == 0 || p->scratch || split_of(p->B, p->T, p->D, grad).bytes == 0, PA_ERR_INVALID,
              "%s: this shape needs scratch (pa_gated_recurrence_scratch)", who);
   return PA_OK;
 }
 
 }  // namespace
 
-extern "C" int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D, int32_t dtype) {
-  return B <= 0 || T <= 0 || D <= 0 || !elem_size(dtype) ? 0 : split_of(B, T, D, dtype).bytes;
+extern "C" int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D) {
+  if (B <= 0 || T <= 0 || D <= 0) return 0;
+  const int64_t forward = split_of(B, T, D, false).bytes, grad = split_of(B, T, D, true).bytes;
+  return forward > grad ? forward : grad;
 }
 
 extern "C" int64_t pa_gated_recurrence_carries(int64_t B, int64_t T, int32_t D) {
-  return B <= 0 || T <= 0 || D <= 0 ? 0 : B * ceil_div(T, tile_steps(T)) * D;
+  return B <= 0 || T <= 0 || D <= 0 ? 0 : B * split_of(B, T, D, true).tiles * D;
 }
 
 extern "C" int pa_gated_recurrence(const pa_recurrence_args* args, void* stream) {
-  const int rc = check_args("pa_gated_recurrence", args);
+  const int rc = check_args("pa_gated_recurrence", args, false);
   if (rc != PA_OK) return rc;
   if (args->B == 0) return PA_OK;
   PA_REQUIRE(args->h, PA_ERR_INVALID, "pa_gated_recurrence: null output");
@@ -665,7 +918,7 @@ extern "C" int pa_gated_recurrence(const pa_recurrence_args* args, void* stream)
 }
 
 extern "C" int pa_gated_recurrence_grad(const pa_recurrence_args* args, void* stream) {
-  const int rc = check_args("pa_gated_recurrence_grad", args);
+  const int rc = check_args("pa_gated_recurrence_grad", args, true);
   if (rc != PA_OK) return rc;
   if (args->B == 0) return PA_OK;
   PA_REQUIRE(args->carries && args->d_x && args->d_gate, PA_ERR_INVALID,

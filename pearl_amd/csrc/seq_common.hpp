@@ -1,5 +1,5 @@
 // Shared by the token-policy operators (embed.hip, recurrence.hip, log_probs.hip): element types,
-// 16-byte accesses at element alignment, and the device guard of their C entries.
+// wide accesses at element alignment, and the device guard of their C entries.
 #pragma once
 #include "common.hpp"
 
@@ -50,30 +50,36 @@ struct Pack {
   uint32_t w[WORDS];
 };
 
-template <int BYTES> struct Words;
-template <> struct Words<4> { typedef uint32_t U __attribute__((ext_vector_type(4), aligned(4), may_alias)); };
-template <> struct Words<2> { typedef uint32_t U __attribute__((ext_vector_type(4), aligned(2), may_alias)); };
+template <int BYTES, int N> struct Words;
+template <> struct Words<4, 4> { typedef uint32_t U __attribute__((ext_vector_type(4), aligned(4), may_alias)); };
+template <> struct Words<2, 4> { typedef uint32_t U __attribute__((ext_vector_type(4), aligned(2), may_alias)); };
+template <> struct Words<4, 2> { typedef uint32_t U __attribute__((ext_vector_type(2), aligned(4), may_alias)); };
+template <> struct Words<2, 1> { typedef uint32_t U __attribute__((ext_vector_type(1), aligned(2), may_alias)); };
+template <> struct Words<2, 2> { typedef uint32_t U __attribute__((ext_vector_type(2), aligned(2), may_alias)); };
 
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
-  typedef typename Words<(int)sizeof(T)>::U U;
+  constexpr int W = Pack<T, N>::WORDS < 4 ? Pack<T, N>::WORDS : 4;      // words per access
+  typedef typename Words<(int)sizeof(T), W>::U U;
   Pack<T, N> r;
-  static_assert(Pack<T, N>::WORDS % 4 == 0, "whole 16-byte accesses");
 #pragma unroll
-  for (int i = 0; i < Pack<T, N>::WORDS; i += 4) {
+  for (int i = 0; i < Pack<T, N>::WORDS; i += W) {
     const U u = *reinterpret_cast<const U*>(p + i * 4 / (int)sizeof(T));
-    r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
+#pragma unroll
+    for (int k = 0; k < W; ++k) r.w[i + k] = u[k];
   }
   return r;
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
-  typedef typename Words<(int)sizeof(T)>::U U;
+  constexpr int W = Pack<T, N>::WORDS < 4 ? Pack<T, N>::WORDS : 4;
+  typedef typename Words<(int)sizeof(T), W>::U U;
 #pragma unroll
-  for (int i = 0; i < Pack<T, N>::WORDS; i += 4) {
+  for (int i = 0; i < Pack<T, N>::WORDS; i += W) {
     U u;
-    u.x = r.w[i]; u.y = r.w[i + 1]; u.z = r.w[i + 2]; u.w = r.w[i + 3];
+#pragma unroll
+    for (int k = 0; k < W; ++k) u[k] = r.w[i + k];
     *reinterpret_cast<U*>(p + i * 4 / (int)sizeof(T)) = u;
   }
 }

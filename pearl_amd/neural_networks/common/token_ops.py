@@ -143,7 +143,13 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor] = 
 
 
 def _rows(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """(batch, time, channels) with adjacent channels, and steps less than the kernels' 2^23 bytes apart."""
+    near = t.stride(1) * t.element_size() < 2 ** 23 or t.shape[1] == 1
+    return t if near and (t.stride(2) == 1 or t.shape[2] == 1) else t.contiguous()
+
+
+def _strides(t: Tensor) -> Tuple[int, int]:
+    return t.stride(0), t.stride(1) if t.shape[1] > 1 else 0      # a single step's stride means nothing
 
 
 def _recurrence_args(op: str, x: Tensor, gate: Tensor, initial_state: Optional[Tensor], resets: Optional[Tensor],
@@ -162,8 +168,8 @@ def _recurrence_args(op: str, x: Tensor, gate: Tensor, initial_state: Optional[T
     a.gate_logits, a.reverse = bool(gate_logits), bool(reverse)
     a.B, a.T, a.D = b, t, d
     a.x, a.gate = x.data_ptr(), gate.data_ptr()
-    a.x_b, a.x_t, _ = x.stride()
-    a.gate_b, a.gate_t, _ = gate.stride()
+    a.x_b, a.x_t = _strides(x)
+    a.gate_b, a.gate_t = _strides(gate)
     if initial_state is not None:
         if initial_state.shape != (b, d) or initial_state.dtype != torch.float32:
             raise ValueError(f"{op}: initial_state is {initial_state.dtype} {tuple(initial_state.shape)}, "
@@ -174,7 +180,9 @@ def _recurrence_args(op: str, x: Tensor, gate: Tensor, initial_state: Optional[T
         if resets.shape != (b, t) or resets.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"{op}: resets is {resets.dtype} {tuple(resets.shape)}, not bool {(b, t)}")
         a.resets = resets.data_ptr()
-        a.resets_b, a.resets_t = resets.stride()
+        if resets.stride(1) >= 2 ** 23:
+            resets = resets.contiguous()
+        a.resets_b, a.resets_t = _strides(resets)
     if lengths is not None:
         if lengths.shape != (b,) or lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{op}: lengths is {lengths.dtype} {tuple(lengths.shape)}, not int32 or int64 {(b,)}")
@@ -204,7 +212,7 @@ def _recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor], resets
     if keep:
         kept = torch.empty(lib.pa_gated_recurrence_carries(b, t, d), dtype=torch.float32, device=device)
         a.carries = kept.data_ptr()
-    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d, a.dtype), device)
+    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d), device)
     a.scratch = N.ptr(scratch)
     N.check(lib.pa_gated_recurrence(byref(a), N.stream_ptr(device)))
     del alive
@@ -230,7 +238,7 @@ def gated_recurrence_grad(x: Tensor, gate: Tensor, kept: Tensor, d_h: Optional[T
     if d_h is not None:
         d_h = _rows(d_h)
         a.d_h = d_h.data_ptr()
-        a.d_h_b, a.d_h_t, _ = d_h.stride()
+        a.d_h_b, a.d_h_t = _strides(d_h)
     if d_last is not None:
         d_last = d_last.contiguous()
         a.d_last = d_last.data_ptr()
@@ -244,7 +252,7 @@ def gated_recurrence_grad(x: Tensor, gate: Tensor, kept: Tensor, d_h: Optional[T
             kept.numel() != lib.pa_gated_recurrence_carries(b, t, d):
         raise ValueError(f"{op}: kept is not what gated_recurrence(..., keep=True) returns for this shape")
     d_h0 = torch.empty(b, d, dtype=torch.float32, device=device)
-    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d, a.dtype), device)
+    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d), device)
     a.carries, a.scratch = kept.data_ptr(), N.ptr(scratch)
     a.d_x, a.d_gate, a.d_h0 = d_x.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr()
     N.check(lib.pa_gated_recurrence_grad(byref(a), N.stream_ptr(device)))
