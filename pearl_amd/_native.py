@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -198,6 +199,8 @@ class MlpDesc(C.Structure):
     ]
 
 
+# Filling a ctypes structure field by field costs more than a small launch: the callers of these two pack
+# their fields, in order, with RECURRENCE_ARGS / LOG_PROBS_ARGS and pass the bytes.
 class RecurrenceArgs(C.Structure):
     _fields_ = [
         ("device", C.c_int32), ("dtype", C.c_int32), ("gate_dtype", C.c_int32),
@@ -225,6 +228,11 @@ class LogProbsArgs(C.Structure):
         ("top_actions", C.c_void_p), ("top_log_probs", C.c_void_p), ("scratch", C.c_void_p),
         ("d_log_prob", C.c_void_p), ("d_entropy", C.c_void_p), ("d_logits", C.c_void_p),
     ]
+
+
+RECURRENCE_ARGS = struct.Struct("6i2qPqqPqqPPqqPPPPPPqqPPPP")
+LOG_PROBS_ARGS = struct.Struct("4iqPqPPqfi9P")
+assert RECURRENCE_ARGS.size == C.sizeof(RecurrenceArgs) and LOG_PROBS_ARGS.size == C.sizeof(LogProbsArgs)
 
 
 class DsacStepArgs(C.Structure):
@@ -436,11 +444,11 @@ SIGNATURES = {
                                        C.c_int32, _P, _P, C.c_int32, _P]),
     "pa_gated_recurrence_scratch": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
     "pa_gated_recurrence_carries": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
-    "pa_gated_recurrence": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),
-    "pa_gated_recurrence_grad": (C.c_int, [C.POINTER(RecurrenceArgs), _P]),
+    "pa_gated_recurrence": (C.c_int, [_P, _P]),
+    "pa_gated_recurrence_grad": (C.c_int, [_P, _P]),
     "pa_action_log_probs_scratch": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
-    "pa_action_log_probs": (C.c_int, [C.POINTER(LogProbsArgs), _P]),
-    "pa_action_log_probs_grad": (C.c_int, [C.POINTER(LogProbsArgs), _P]),
+    "pa_action_log_probs": (C.c_int, [_P, _P]),
+    "pa_action_log_probs_grad": (C.c_int, [_P, _P]),
     "pa_one_hot": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int32, _P, _P]),
     "pa_dqn_param_count": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "pa_dqn_param_offsets": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),

@@ -12,7 +12,7 @@ a backward pass when gradients are asked for; ``embed_tokens_grad`` and ``gated_
 the same kernels for learners that run their backward pass explicitly."""
 from __future__ import annotations
 
-from ctypes import byref
+from functools import lru_cache
 from typing import Any, Optional, Tuple
 
 import torch
@@ -47,8 +47,8 @@ def scratch_of(nbytes: int, device: torch.device) -> Optional[Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def wants_grad(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _address(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------- embedding
@@ -59,7 +59,7 @@ def embed_tokens(weight: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
     Token -1 stands for "none": a row of zeros that takes no part in the gradient.  Any other token
     outside the table gives a row of NaN; nothing is read for it.  The weight's gradient is dense,
     summed in float32 in the order of the tokens and the same bits for the same inputs."""
-    if wants_grad(weight):
+    if weight.requires_grad and torch.is_grad_enabled():
         return _EmbedTokens.apply(weight, tokens, scale)
     return _embed(weight, tokens, scale)
 
@@ -136,7 +136,8 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor] = 
 
     Returns ``(h, last_state)``.  With ``keep=True`` no backward pass is recorded and a third result is
     what ``gated_recurrence_grad`` needs of the forward pass."""
-    if not keep and wants_grad(x, gate, initial_state):
+    if not keep and torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
+            initial_state is not None and initial_state.requires_grad)):
         return _GatedRecurrence.apply(x, gate, initial_state, resets, lengths, gate_logits, reverse)
     h, last, kept = _recurrence(x, gate, initial_state, resets, lengths, gate_logits, reverse, keep)
     return (h, last, kept) if keep else (h, last)
@@ -152,70 +153,65 @@ def _strides(t: Tensor) -> Tuple[int, int]:
     return t.stride(0), t.stride(1) if t.shape[1] > 1 else 0      # a single step's stride means nothing
 
 
-def _recurrence_args(op: str, x: Tensor, gate: Tensor, initial_state: Optional[Tensor], resets: Optional[Tensor],
-                     lengths: Optional[Tensor], gate_logits: bool, reverse: bool, a: N.RecurrenceArgs) -> Tuple:
-    """Checks the arguments that both directions share and fills them in; returns what must stay alive."""
-    device = x.device
+@lru_cache(maxsize=4096)
+def _recurrence_sizes(b: int, t: int, d: int) -> Tuple[int, int]:
+    """Scratch bytes of a call and floats kept for its gradient."""
+    lib = N.lib()
+    return lib.pa_gated_recurrence_scratch(b, t, d), lib.pa_gated_recurrence_carries(b, t, d)
+
+
+def _inputs(op: str, x: Tensor, gate: Tensor, resets: Optional[Tensor], lengths: Optional[Tensor]) -> Tuple:
+    """Checks what both directions share; returns it as the kernels take it, with the dtypes' codes."""
     if x.dim() != 3 or gate.shape != x.shape:
         raise ValueError(f"{op}: x has shape {tuple(x.shape)} and gate {tuple(gate.shape)}, "
                          "not twice (batch, time, channels)")
-    a.dtype = dtype_code(op, "x", x, FLOATS)
-    a.gate_dtype = dtype_code(op, "gate", gate, FLOATS)
-    if gate.dtype != x.dtype and gate.dtype != torch.float32:
+    code, gate_code = dtype_code(op, "x", x, FLOATS), dtype_code(op, "gate", gate, FLOATS)
+    if gate_code != code and gate_code != N.PA_F32:
         raise TypeError(f"{op}: gate is {gate.dtype}, x is {x.dtype}: the gate has x's type or float32")
-    b, t, d = x.shape
-    x, gate = _rows(x), _rows(gate)
-    a.gate_logits, a.reverse = bool(gate_logits), bool(reverse)
-    a.B, a.T, a.D = b, t, d
-    a.x, a.gate = x.data_ptr(), gate.data_ptr()
-    a.x_b, a.x_t = _strides(x)
-    a.gate_b, a.gate_t = _strides(gate)
-    if initial_state is not None:
-        if initial_state.shape != (b, d) or initial_state.dtype != torch.float32:
-            raise ValueError(f"{op}: initial_state is {initial_state.dtype} {tuple(initial_state.shape)}, "
-                             f"not float32 {(b, d)}")
-        initial_state = initial_state.contiguous()
-        a.h0 = initial_state.data_ptr()
+    b, t, _ = x.shape
     if resets is not None:
         if resets.shape != (b, t) or resets.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"{op}: resets is {resets.dtype} {tuple(resets.shape)}, not bool {(b, t)}")
-        a.resets = resets.data_ptr()
         if resets.stride(1) >= 2 ** 23:
             resets = resets.contiguous()
-        a.resets_b, a.resets_t = _strides(resets)
     if lengths is not None:
         if lengths.shape != (b,) or lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{op}: lengths is {lengths.dtype} {tuple(lengths.shape)}, not int32 or int64 {(b,)}")
+        on_one_gpu(op, x.device, lengths)
         # clamped before the cast, so that no length wraps around
-        on_one_gpu(op, device, lengths)
         lengths = (lengths.clamp(0, t).to(torch.int32) if lengths.dtype == torch.int64 else lengths).contiguous()
-        a.lengths = lengths.data_ptr()
-    on_one_gpu(op, device, gate, initial_state, resets)
-    a.device = device.index
-    return x, gate, initial_state, resets, lengths
+    return code, gate_code, _rows(x), _rows(gate), resets, lengths
+
+
+def _check_state(op: str, name: str, state: Tensor, shape: Tuple[int, int]) -> Tensor:
+    if state.shape != shape or state.dtype != torch.float32:
+        raise ValueError(f"{op}: {name} is {state.dtype} {tuple(state.shape)}, not float32 {shape}")
+    return state.contiguous()
 
 
 def _recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor], resets: Optional[Tensor],
                 lengths: Optional[Tensor], gate_logits: bool, reverse: bool, keep: bool) -> Tuple:
-    a = N.RecurrenceArgs()
-    alive = _recurrence_args("gated_recurrence", x, gate, initial_state, resets, lengths, gate_logits, reverse, a)
+    op = "gated_recurrence"
+    code, gate_code, xs, gs, resets, lengths = _inputs(op, x, gate, resets, lengths)
     b, t, d = x.shape
+    if initial_state is not None:
+        initial_state = _check_state(op, "initial_state", initial_state, (b, d))
     device = x.device
+    on_one_gpu(op, device, gate, initial_state, resets)
     h = torch.empty(b, t, d, dtype=x.dtype, device=device)
     if b * t * d == 0:      # no step: the state passes through
         last = torch.zeros(b, d, device=device) if initial_state is None else initial_state.detach().clone()
         return h, last, torch.empty(0, device=device)
-    lib = N.lib()
+    scratch_bytes, carries = _recurrence_sizes(b, t, d)
     last = torch.empty(b, d, dtype=torch.float32, device=device)
-    a.h, a.last = h.data_ptr(), last.data_ptr()
-    kept = None
-    if keep:
-        kept = torch.empty(lib.pa_gated_recurrence_carries(b, t, d), dtype=torch.float32, device=device)
-        a.carries = kept.data_ptr()
-    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d), device)
-    a.scratch = N.ptr(scratch)
-    N.check(lib.pa_gated_recurrence(byref(a), N.stream_ptr(device)))
-    del alive
+    kept = torch.empty(carries, dtype=torch.float32, device=device) if keep else None
+    scratch = scratch_of(scratch_bytes, device)
+    args = N.RECURRENCE_ARGS.pack(
+        device.index, code, gate_code, bool(gate_logits), bool(reverse), d, b, t,
+        xs.data_ptr(), *_strides(xs), gs.data_ptr(), *_strides(gs), _address(initial_state),
+        _address(resets), *((0, 0) if resets is None else _strides(resets)), _address(lengths),
+        h.data_ptr(), last.data_ptr(), _address(kept), _address(scratch), 0, 0, 0, 0, 0, 0, 0)
+    N.check(N.lib().pa_gated_recurrence(args, N.stream_ptr(device)))
     return h, last, kept
 
 
@@ -226,37 +222,33 @@ def gated_recurrence_grad(x: Tensor, gate: Tensor, kept: Tensor, d_h: Optional[T
     """Gradients ``(d_x, d_gate, d_initial_state)`` of ``gated_recurrence`` called with ``keep=True`` on the
     same x, gate, resets, lengths and flags, for the gradients of h and of the last state (None: zero)."""
     op = "gated_recurrence_grad"
-    if d_h is not None and (d_h.shape != x.shape or d_h.dtype != x.dtype):
-        raise ValueError(f"{op}: d_h is {d_h.dtype} {tuple(d_h.shape)}, not {x.dtype} {tuple(x.shape)}")
-    if d_last is not None and (d_last.shape != x.shape[:1] + x.shape[-1:] or d_last.dtype != torch.float32):
-        raise ValueError(f"{op}: d_last is {d_last.dtype} {tuple(d_last.shape)}, not float32 (batch, channels)")
-    a = N.RecurrenceArgs()
-    alive = _recurrence_args(op, x, gate, None, resets, lengths, gate_logits, reverse, a)
+    code, gate_code, xs, gs, resets, lengths = _inputs(op, x, gate, resets, lengths)
     b, t, d = x.shape
-    device = x.device
-    on_one_gpu(op, device, d_h, d_last, kept)
     if d_h is not None:
+        if d_h.shape != x.shape or d_h.dtype != x.dtype:
+            raise ValueError(f"{op}: d_h is {d_h.dtype} {tuple(d_h.shape)}, not {x.dtype} {tuple(x.shape)}")
         d_h = _rows(d_h)
-        a.d_h = d_h.data_ptr()
-        a.d_h_b, a.d_h_t = _strides(d_h)
     if d_last is not None:
-        d_last = d_last.contiguous()
-        a.d_last = d_last.data_ptr()
+        d_last = _check_state(op, "d_last", d_last, (b, d))
+    device = x.device
+    on_one_gpu(op, device, gate, resets, d_h, d_last, kept)
     d_x = torch.empty(b, t, d, dtype=x.dtype, device=device)
     d_gate = torch.empty(b, t, d, dtype=gate.dtype, device=device)
     if b * t * d == 0:
         d_h0 = torch.zeros(b, d, device=device) if d_last is None else d_last.clone()
         return d_x, d_gate, d_h0
-    lib = N.lib()
-    if kept.dtype != torch.float32 or not kept.is_contiguous() or \
-            kept.numel() != lib.pa_gated_recurrence_carries(b, t, d):
+    scratch_bytes, carries = _recurrence_sizes(b, t, d)
+    if kept.dtype != torch.float32 or not kept.is_contiguous() or kept.numel() != carries:
         raise ValueError(f"{op}: kept is not what gated_recurrence(..., keep=True) returns for this shape")
     d_h0 = torch.empty(b, d, dtype=torch.float32, device=device)
-    scratch = scratch_of(lib.pa_gated_recurrence_scratch(b, t, d), device)
-    a.carries, a.scratch = kept.data_ptr(), N.ptr(scratch)
-    a.d_x, a.d_gate, a.d_h0 = d_x.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr()
-    N.check(lib.pa_gated_recurrence_grad(byref(a), N.stream_ptr(device)))
-    del alive
+    scratch = scratch_of(scratch_bytes, device)
+    args = N.RECURRENCE_ARGS.pack(
+        device.index, code, gate_code, bool(gate_logits), bool(reverse), d, b, t,
+        xs.data_ptr(), *_strides(xs), gs.data_ptr(), *_strides(gs), 0,
+        _address(resets), *((0, 0) if resets is None else _strides(resets)), _address(lengths),
+        0, 0, kept.data_ptr(), _address(scratch), _address(d_h), *((0, 0) if d_h is None else _strides(d_h)),
+        _address(d_last), d_x.data_ptr(), d_gate.data_ptr(), d_h0.data_ptr())
+    N.check(N.lib().pa_gated_recurrence_grad(args, N.stream_ptr(device)))
     return d_x, d_gate, d_h0
 
 
@@ -290,26 +282,38 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
     channels) or None for zeros, resets (batch).  Returns ``(h, new_state)``; ``out_state`` receives the new
     state and may be ``state`` itself.  Records no backward pass and refuses inputs that ask for one."""
     op = "gated_recurrence_step"
-    if wants_grad(x, gate, state):
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
+            state is not None and state.requires_grad)):
         raise RuntimeError(f"{op} records no backward pass: call it under torch.no_grad(), or gated_recurrence")
-    if x.dim() != 2 or gate.shape != x.shape:
+    shape = x.shape
+    if len(shape) != 2 or gate.shape != shape:
         raise ValueError(f"{op}: x has shape {tuple(x.shape)} and gate {tuple(gate.shape)}, "
                          "not twice (batch, channels)")
-    if resets is not None and resets.shape != x.shape[:1]:
-        raise ValueError(f"{op}: resets has shape {tuple(resets.shape)}, not {tuple(x.shape[:1])}")
-    a = N.RecurrenceArgs()
-    alive = _recurrence_args(op, x.unsqueeze(1), gate.unsqueeze(1), state,
-                             None if resets is None else resets.unsqueeze(1), None, gate_logits, False, a)
-    b, d = x.shape
+    code, gate_code = dtype_code(op, "x", x, FLOATS), dtype_code(op, "gate", gate, FLOATS)
+    if gate_code != code and gate_code != N.PA_F32:
+        raise TypeError(f"{op}: gate is {gate.dtype}, x is {x.dtype}: the gate has x's type or float32")
+    b, d = shape
+    if state is not None:
+        state = _check_state(op, "state", state, shape)
+    if resets is not None and (resets.shape != shape[:1] or resets.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"{op}: resets is {resets.dtype} {tuple(resets.shape)}, not bool {(b,)}")
+    if out_state is not None and (out_state.shape != shape or out_state.dtype != torch.float32
+                                  or not out_state.is_contiguous()):
+        raise ValueError(f"{op}: out_state is not a contiguous float32 tensor of shape {(b, d)}")
+    device = x.device
+    on_one_gpu(op, device, gate, state, resets, out_state)
+    if x.stride(1) != 1 and d > 1:
+        x = x.contiguous()
+    if gate.stride(1) != 1 and d > 1:
+        gate = gate.contiguous()
+    h = torch.empty(b, d, dtype=x.dtype, device=device)
     if out_state is None:
-        out_state = torch.empty(b, d, dtype=torch.float32, device=x.device)
-    else:
-        on_one_gpu(op, x.device, out_state)
-        if out_state.shape != (b, d) or out_state.dtype != torch.float32 or not out_state.is_contiguous():
-            raise ValueError(f"{op}: out_state is not a contiguous float32 tensor of shape {(b, d)}")
-    h = torch.empty(b, d, dtype=x.dtype, device=x.device)
+        out_state = torch.empty(b, d, dtype=torch.float32, device=device)
     if b * d:
-        a.h, a.last = h.data_ptr(), out_state.data_ptr()
-        N.check(N.lib().pa_gated_recurrence(byref(a), N.stream_ptr(x.device)))
-    del alive
+        args = N.RECURRENCE_ARGS.pack(
+            device.index, code, gate_code, bool(gate_logits), False, d, b, 1,
+            x.data_ptr(), x.stride(0), 0, gate.data_ptr(), gate.stride(0), 0, _address(state),
+            _address(resets), 0 if resets is None else resets.stride(0), 0, 0,
+            h.data_ptr(), out_state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        N.check(N.lib().pa_gated_recurrence(args, N.stream_ptr(device)))
     return h, out_state

@@ -3,7 +3,7 @@ best alternatives: ``VanillaActorNetwork.get_action_prob`` (actor_networks.py:15
 any number of actions, from the logits (``pa_action_log_probs``, log_probs.hip)."""
 from __future__ import annotations
 
-from ctypes import byref
+from functools import lru_cache
 from typing import Any, NamedTuple, Optional, Tuple
 
 import torch
@@ -11,7 +11,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ... import _native as N
-from ..common.token_ops import FLOATS, INDICES, dtype_code, on_one_gpu, scratch_of, wants_grad
+from ..common.token_ops import FLOATS, INDICES, _address, dtype_code, on_one_gpu, scratch_of
 
 
 class ActionLogProbs(NamedTuple):
@@ -32,67 +32,68 @@ def action_log_probs(logits: Tensor, actions: Tensor, unavailable_actions_mask: 
     A row without an available action has log_prob -inf, entropy 0, alternatives -1.  Action -1 stands for
     "none taken" (padding): log_prob 0.  Any other action outside [0, A) gives NaN.  log_prob and entropy are
     differentiable with respect to the logits; the alternatives are not."""
-    if wants_grad(logits):
+    if logits.requires_grad and torch.is_grad_enabled():
         out = _ActionLogProbs.apply(logits, actions, unavailable_actions_mask, temperature, top)
         return ActionLogProbs(*out)
     return _log_probs(logits, actions, unavailable_actions_mask, temperature, top)
 
 
-def _args(op: str, logits: Tensor, actions: Tensor, mask: Optional[Tensor], temperature: float) -> Tuple:
-    device = logits.device
-    if logits.dim() < 1 or logits.shape[:-1] != actions.shape:
+@lru_cache(maxsize=4096)
+def _scratch_bytes(rows: int, width: int, code: int, top: int) -> int:
+    return N.lib().pa_action_log_probs_scratch(rows, width, code, top)
+
+
+def _inputs(op: str, logits: Tensor, actions: Tensor, mask: Optional[Tensor], temperature: float) -> Tuple:
+    """Checks what both directions share; returns the head of the C arguments and what it points to."""
+    shape = logits.shape
+    if not shape or shape[:-1] != actions.shape:
         raise ValueError(f"{op}: logits have shape {tuple(logits.shape)}, actions {tuple(actions.shape)}, "
                          "not (..., A) and (...)")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"{op}: temperature {temperature}")
-    a = N.LogProbsArgs()
-    a.dtype = dtype_code(op, "logits", logits, FLOATS)
-    a.action_dtype = dtype_code(op, "actions", actions, INDICES)
-    width = logits.shape[-1]
-    rows = actions.numel()
-    flat = logits if logits.dim() == 2 else logits.reshape(rows, width)
+    code, action_code = dtype_code(op, "logits", logits, FLOATS), dtype_code(op, "actions", actions, INDICES)
+    width, rows = shape[-1], actions.numel()
+    flat = logits if len(shape) == 2 else logits.reshape(rows, width)
     if flat.stride(1) != 1 and width > 1:
         flat = flat.contiguous()
     actions = actions.contiguous()
-    a.A, a.rows, a.temperature = width, rows, temperature
-    a.logits, a.ld, a.actions = flat.data_ptr(), flat.stride(0), actions.data_ptr()
+    mask_ld = 0
     if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8) or (mask.shape != logits.shape and mask.shape != (width,)):
+        if mask.dtype not in (torch.bool, torch.uint8) or (mask.shape != shape and mask.shape != shape[-1:]):
             raise ValueError(f"{op}: unavailable_actions_mask is {mask.dtype} {tuple(mask.shape)}, "
-                             f"not bool {tuple(logits.shape)} or {(width,)}")
-        if mask.dim() == 1 and logits.dim() != 1:
+                             f"not bool {tuple(shape)} or {(width,)}")
+        if mask.dim() == 1 and len(shape) != 1:
             mask = mask.contiguous()
         else:
-            mask = mask.reshape(rows, width)
+            mask = mask if len(shape) == 2 else mask.reshape(rows, width)
             if mask.stride(1) != 1 and width > 1:
                 mask = mask.contiguous()
-            a.ldm = mask.stride(0)
-        a.mask = mask.data_ptr()
+            mask_ld = mask.stride(0)
+    device = logits.device
     on_one_gpu(op, device, actions, mask)
-    a.device = device.index
-    return a, (flat, actions, mask)
+    head = (device.index, code, action_code, width, rows, flat.data_ptr(), flat.stride(0), actions.data_ptr(),
+            _address(mask), mask_ld, temperature)
+    return head, (flat, actions, mask)
 
 
 def _log_probs(logits: Tensor, actions: Tensor, mask: Optional[Tensor], temperature: float, top: int
                ) -> ActionLogProbs:
     if not 0 <= top <= 64:
         raise NotImplementedError(f"action_log_probs: top {top} (0 to 64)")
-    a, alive = _args("action_log_probs", logits, actions, mask, temperature)
+    head, alive = _inputs("action_log_probs", logits, actions, mask, temperature)
     device, shape = logits.device, actions.shape
-    a.top = top
-    log_prob = torch.empty(shape, dtype=torch.float32, device=device)
-    entropy = torch.empty(shape, dtype=torch.float32, device=device)
-    stats = torch.empty(*shape, 3, dtype=torch.float32, device=device)
+    f32 = torch.float32
+    log_prob = torch.empty(shape, dtype=f32, device=device)
+    entropy = torch.empty(shape, dtype=f32, device=device)
+    stats = torch.empty(*shape, 3, dtype=f32, device=device)
     top_actions = top_log_probs = None
     if top:
         top_actions = torch.empty(*shape, top, dtype=torch.int64, device=device)
-        top_log_probs = torch.empty(*shape, top, dtype=torch.float32, device=device)
-        a.top_actions, a.top_log_probs = top_actions.data_ptr(), top_log_probs.data_ptr()
-    lib = N.lib()
-    scratch = scratch_of(lib.pa_action_log_probs_scratch(a.rows, a.A, a.dtype, top), device)
-    a.log_prob, a.entropy, a.stats = log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
-    a.scratch = N.ptr(scratch)
-    N.check(lib.pa_action_log_probs(byref(a), N.stream_ptr(device)))
+        top_log_probs = torch.empty(*shape, top, dtype=f32, device=device)
+    scratch = scratch_of(_scratch_bytes(head[4], head[3], head[1], top), device)
+    args = N.LOG_PROBS_ARGS.pack(*head, top, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                 _address(top_actions), _address(top_log_probs), _address(scratch), 0, 0, 0)
+    N.check(N.lib().pa_action_log_probs(args, N.stream_ptr(device)))
     del alive
     return ActionLogProbs(log_prob, entropy, top_actions, top_log_probs, stats)
 
@@ -103,23 +104,20 @@ def action_log_probs_grad(out: ActionLogProbs, logits: Tensor, actions: Tensor,
     """The logits' gradient, in their type, of ``action_log_probs`` called with the same arguments, for the
     float32 gradients of log_prob and of the entropy (None: zero)."""
     op = "action_log_probs_grad"
-    a, alive = _args(op, logits, actions, unavailable_actions_mask, temperature)
-    device, shape = logits.device, actions.shape
-    stats = out.row_stats
+    head, alive = _inputs(op, logits, actions, unavailable_actions_mask, temperature)
+    device, shape, stats = logits.device, actions.shape, out.row_stats
     on_one_gpu(op, device, stats, d_log_prob, d_entropy)
     if stats.shape != (*shape, 3) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError(f"{op}: out.row_stats is not what action_log_probs returns for these logits")
-    grads = []
     for name, t in (("d_log_prob", d_log_prob), ("d_entropy", d_entropy)):
-        if t is not None:
-            if t.shape != shape or t.dtype != torch.float32:
-                raise ValueError(f"{op}: {name} is {t.dtype} {tuple(t.shape)}, not float32 {tuple(shape)}")
-            t = t.contiguous()
-        grads.append(t)
+        if t is not None and (t.shape != shape or t.dtype != torch.float32):
+            raise ValueError(f"{op}: {name} is {t.dtype} {tuple(t.shape)}, not float32 {tuple(shape)}")
+    d_log_prob = None if d_log_prob is None else d_log_prob.contiguous()
+    d_entropy = None if d_entropy is None else d_entropy.contiguous()
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    a.stats = stats.data_ptr()
-    a.d_log_prob, a.d_entropy, a.d_logits = N.ptr(grads[0]), N.ptr(grads[1]), d_logits.data_ptr()
-    N.check(N.lib().pa_action_log_probs_grad(byref(a), N.stream_ptr(device)))
+    args = N.LOG_PROBS_ARGS.pack(*head, 0, 0, 0, stats.data_ptr(), 0, 0, 0, _address(d_log_prob), _address(d_entropy),
+                                 d_logits.data_ptr())
+    N.check(N.lib().pa_action_log_probs_grad(args, N.stream_ptr(device)))
     del alive
     return d_logits
 

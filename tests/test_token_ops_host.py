@@ -25,6 +25,7 @@ def test_ctypes_structs_match_the_header(tmp_path):
     (tmp_path / "probe.c").write_text("\n".join(src))
     subprocess.run(["gcc", "-std=c99", "-o", str(tmp_path / "probe"), str(tmp_path / "probe.c")], check=True)
     lines = subprocess.run([str(tmp_path / "probe")], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert N.RECURRENCE_ARGS.size == C.sizeof(N.RecurrenceArgs) and N.LOG_PROBS_ARGS.size == C.sizeof(N.LogProbsArgs)
     for s, line in zip(pairs.values(), lines):
         assert [int(v) for v in line.split()] == [C.sizeof(s)] + [getattr(s, f[0]).offset for f in s._fields_]
 
