@@ -27,6 +27,7 @@ from .neural_networks.common.token_ops import (embed_tokens, embed_tokens_grad, 
 from .neural_networks.sequential_decision_making.action_log_probs import (ActionLogProbs,  # noqa: F401
                                                                           action_log_probs,
                                                                           action_log_probs_grad)
+from .neural_networks.sequential_decision_making.actor_networks import RecurrentActorNetwork  # noqa: F401
 from .vector_env import BatchedActionResult, BatchedEnvironment, VectorEnvFeeder  # noqa: F401
 
 __version__ = "0.1.0"

@@ -8,6 +8,7 @@ the softmax / tanh-Gaussian heads of libpearl_amd (``pa_softmax_action_prob``,
 ``pa_gauss_sample``).  The torch expressions below serve ``act()`` (outside the measured path)."""
 from __future__ import annotations
 
+import math
 from typing import Any, List, Optional, Tuple, Union
 
 import torch
@@ -15,7 +16,9 @@ import torch.nn as nn
 from torch import Tensor
 from torch.distributions import Normal
 
+from ..common.token_ops import embed_tokens, gated_recurrence, gated_recurrence_step
 from ..common.utils import mlp_block, linear_layers_of_plain
+from .action_log_probs import ActionLogProbs, action_log_probs
 
 
 def action_scaling(action_space: Any, input_action: Tensor) -> Tensor:
@@ -140,3 +143,60 @@ class GaussianActorNetwork(ActorNetwork):
 
     def trunk_layers(self) -> List[nn.Linear]:
         return linear_layers_of_plain(self._model, type(self).__name__)
+
+
+class RecurrentActorNetwork(ActorNetwork):
+    """Softmax policy over a discrete action set, given a history of tokens (discrete observations, or the
+    actions and observations of an episode written as one sequence).
+
+    Embedding -> gated linear recurrence -> linear head, on HIP (``embed_tokens``,
+    ``gated_recurrence``, ``action_log_probs``) with the two dense layers as library products.  ``input_dim`` is
+    the number of tokens, ``hidden_dims`` holds one width.  Trains through autograd; the parameters may be
+    float32, bfloat16 or float16, the recurrent state is float32.
+
+    The fused learners (PPO, SAC, ...) hard-wire multilayer perceptrons and refuse it."""
+
+    def __init__(self, input_dim: int, hidden_dims: Optional[List[int]], output_dim: int,
+                 action_space: Any = None) -> None:
+        super().__init__(input_dim, hidden_dims, output_dim, action_space)
+        if hidden_dims is None or len(hidden_dims) != 1:
+            raise ValueError("RecurrentActorNetwork takes one hidden dim: the width of its recurrence")
+        self._hidden = int(hidden_dims[0])
+        # rows of variance 1 / hidden, scaled to variance 1 at the lookup
+        self._embedding = nn.Parameter(torch.randn(input_dim, self._hidden) / math.sqrt(self._hidden))
+        self._inputs = nn.Linear(self._hidden, 2 * self._hidden)      # candidate states | gate logits
+        self._head = nn.Linear(self._hidden, output_dim)
+        with torch.no_grad():
+            self._inputs.bias[self._hidden:].fill_(2.0)               # remember about eight steps at first
+
+    def initial_state(self, batch: int) -> Tensor:
+        return torch.zeros(batch, self._hidden, dtype=torch.float32, device=self._embedding.device)
+
+    def forward(self, tokens: Tensor, state: Optional[Tensor] = None, resets: Optional[Tensor] = None,
+                lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """Logits (batch, time, actions) after every token and the state behind the last one.  ``resets``
+        marks the tokens that begin an episode, ``lengths`` ends padded histories (token -1 pads)."""
+        both = self._inputs(embed_tokens(self._embedding, tokens, scale=math.sqrt(self._hidden)))
+        x, gate = both.split(self._hidden, dim=-1)
+        h, last = gated_recurrence(x, gate, state, resets=resets, lengths=lengths)
+        return self._head(h), last
+
+    def step(self, tokens: Tensor, state: Tensor, resets: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """Logits (batch, actions) after one more token each, and the new state; for acting, no gradients."""
+        with torch.no_grad():
+            both = self._inputs(embed_tokens(self._embedding, tokens, scale=math.sqrt(self._hidden)))
+            x, gate = both.split(self._hidden, dim=-1)
+            h, state = gated_recurrence_step(x, gate, state, resets=resets)
+            return self._head(h), state
+
+    def get_log_probs(self, tokens: Tensor, action_batch: Tensor, state: Optional[Tensor] = None,
+                      resets: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+                      unavailable_actions_mask: Optional[Tensor] = None, temperature: float = 1.0, top: int = 0
+                      ) -> Tuple[ActionLogProbs, Tensor]:
+        """log pi(action | history) and the policy's entropy after every token, and the last state."""
+        logits, last = self.forward(tokens, state, resets, lengths)
+        return action_log_probs(logits, action_batch, unavailable_actions_mask, temperature, top), last
+
+    def linear_layers(self) -> List[nn.Linear]:
+        raise NotImplementedError("pearl_amd: RecurrentActorNetwork is not a multilayer perceptron: the fused "
+                                  "learners cannot train it; it trains through autograd")

@@ -396,6 +396,79 @@ def test_action_log_probs_autograd():
         assert torch.isfinite(leaf.grad).all()
 
 
+# ---------------------------------------------------------------------------- the policy they make up
+def plain_policy(net, tokens, actions, state, resets, lengths, mask):
+    """RecurrentActorNetwork.get_log_probs in torch, 64 bits, on the CPU; a loop over the steps."""
+    p = {k: v.detach().double().cpu().requires_grad_() for k, v in net.named_parameters()}
+    hidden = p["_head.weight"].shape[1]
+    e = p["_embedding"][tokens.clamp(min=0)] * math.sqrt(hidden) * (tokens >= 0)[..., None]
+    both = e @ p["_inputs.weight"].t() + p["_inputs.bias"]
+    x, a = both[..., :hidden], torch.sigmoid(both[..., hidden:])
+    h, outs = state, []
+    for t in range(tokens.shape[1]):
+        on = (t < lengths)[:, None]
+        new = a[:, t] * torch.where(resets[:, t, None], torch.zeros_like(h), h) + (1 - a[:, t]) * x[:, t]
+        h = torch.where(on, new, h)
+        outs.append(torch.where(on, new, torch.zeros_like(new)))
+    logits = torch.stack(outs, 1) @ p["_head.weight"].t() + p["_head.bias"]
+    log_p = torch.log_softmax(logits.masked_fill(mask, float("-inf")), -1)
+    prob = log_p.exp()
+    entropy = -(prob * torch.where(mask, torch.zeros_like(log_p), log_p)).sum(-1)
+    return p, logits, log_p.gather(-1, actions[..., None])[..., 0], entropy, h
+
+
+@pytest.mark.parametrize("dtype,limit", [(torch.float32, 64 * 48 * O.U), (torch.bfloat16, 2.0 ** -5)], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("batch,time,actions", [(3, 70, 11), (2, 300, 900)])
+def test_recurrent_actor_network(dtype, limit, batch, time, actions):
+    """Forward and gradients of the three operators as one policy.  In fp32 each of four stages forwards
+    and four backwards is off by at most (48 + 50) U of the norms it sums; in bf16 about eight roundings of
+    2^-9 each stand in a row, and parameters are summed over all steps: both limits leave a factor of four
+    for norms that cancel."""
+    from pearl_amd import RecurrentActorNetwork
+    torch.manual_seed(0)
+    net = RecurrentActorNetwork(37, [48], actions).to(DEV, dtype)
+    gen = gen_of(batch, time, actions)
+    tokens = torch.randint(0, 37, (batch, time), generator=gen)
+    lengths = torch.tensor([time, time - 9, 1][:batch])
+    tokens[torch.arange(time)[None] >= lengths[:, None]] = -1
+    acts = torch.randint(0, actions, (batch, time), generator=gen)
+    resets = torch.rand(batch, time, generator=gen) < 0.03
+    mask = torch.rand(batch, time, actions, generator=gen) < 0.2
+    mask.scatter_(-1, acts[..., None], False)
+    state = torch.randn(batch, 48, generator=gen)
+    weight = torch.randn(batch, time, generator=gen) * (torch.arange(time)[None] < lengths[:, None])
+    out, last = net.get_log_probs(tokens.to(DEV), acts.to(DEV), state.to(DEV), resets.to(DEV), lengths.to(DEV),
+                                  mask.to(DEV), top=3)
+    ((out.log_prob + 0.1 * out.entropy) * weight.to(DEV)).sum().backward()
+    p, logits, lp, ent, h = plain_policy(net, tokens, acts, state.double(), resets, lengths, mask)
+    ((lp + 0.1 * ent) * weight.double()).sum().backward()
+    inside = weight != 0
+
+    def off(got, want):
+        return float((got.detach().double().cpu() - want.detach()).norm() / want.detach().norm())
+    assert off(out.log_prob[inside.to(DEV)], lp[inside]) < limit and off(out.entropy[inside.to(DEV)], ent[inside]) < limit
+    assert off(last, h) < limit
+    for name, q in net.named_parameters():
+        assert off(q.grad, p[name].grad) < limit, name
+
+
+def test_recurrent_actor_network_acts_step_by_step_as_it_reads_histories():
+    from pearl_amd import RecurrentActorNetwork
+    torch.manual_seed(1)
+    net = RecurrentActorNetwork(9, [40], 6).to(DEV)
+    tokens = torch.randint(0, 9, (4, 50), device=DEV)
+    resets = torch.rand(4, 50, device=DEV) < 0.1
+    with torch.no_grad():
+        logits, last = net(tokens, resets=resets)
+    state = net.initial_state(4)
+    for t in range(50):
+        now, state = net.step(tokens[:, t], state, resets[:, t])
+        torch.testing.assert_close(now, logits[:, t], rtol=0, atol=64 * 40 * O.U * float(logits.abs().max()))
+    torch.testing.assert_close(state, last, rtol=0, atol=64 * 40 * O.U)
+    with pytest.raises(NotImplementedError):
+        net.linear_layers()
+
+
 # ---------------------------------------------------------------------------- streams, graphs, devices
 def a_run(s):
     """The three operators as a policy step uses them; `s` holds its inputs."""

@@ -176,3 +176,15 @@ def test_embedding_gradient_definition_against_differences():
     def loss(w):
         return (np.nan_to_num(O.embed(w, tok, 1.5)[0]) * d).sum()
     np.testing.assert_allclose(O.embed_grad(d, tok, 4, 1.5)[0], _differences(loss, [w], 0), rtol=1e-6, atol=1e-8)
+
+
+def test_recurrent_actor_network_constructor():
+    from pearl_amd import RecurrentActorNetwork
+    net = RecurrentActorNetwork(12, [8], 5)
+    assert sorted(net.state_dict()) == ["_embedding", "_head.bias", "_head.weight", "_inputs.bias", "_inputs.weight"]
+    assert net.initial_state(3).shape == (3, 8)
+    for hidden in (None, [], [4, 4]):
+        with pytest.raises(ValueError):
+            RecurrentActorNetwork(12, hidden, 5)
+    with pytest.raises(NotImplementedError):
+        net.linear_layers()
