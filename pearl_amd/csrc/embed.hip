@@ -71,6 +71,7 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs<T> a) {
 // behind clear d_W meanwhile.
 constexpr int BINS = 512;     // tokens per workgroup
 constexpr int GROUP_WAVES = 16;
+constexpr int AHEAD = 16;     // tokens read at once by a lane
 
 struct GroupArgs {
   const void* tokens; int64_t n;
@@ -106,13 +107,20 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   const int64_t part = (a.n + 64 * GROUP_WAVES - 1) / (64 * GROUP_WAVES) * 64;
   const int64_t i0 = wave * part, i1 = i0 + part < a.n ? i0 + part : a.n;
   uint32_t before = 0, all = 0;
-#pragma unroll 4
-  for (int64_t i = i0 + lane; i < i1; i += 64) {
-    const uint32_t key = token_key(tokens, i, a.vocab);
-    const bool valid = key < a.vocab;
-    before += valid && (key & low) < me;
-    all += valid;
-    if (valid && (key & low) == me) atomicAdd(&count[(key >> a.owner_shift) * GROUP_WAVES + wave], 1u);
+  uint32_t key[AHEAD];
+  for (int64_t g = i0; g < i1; g += 64 * AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t i = g + 64 * u + lane;
+      key[u] = i < i1 ? token_key(tokens, i, a.vocab) : a.vocab;
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const bool valid = key[u] < a.vocab;
+      before += valid && (key[u] & low) < me;
+      all += valid;
+      if (valid && (key[u] & low) == me) atomicAdd(&count[(key[u] >> a.owner_shift) * GROUP_WAVES + wave], 1u);
+    }
   }
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
@@ -155,24 +163,31 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
     }
   }
   __syncthreads();
-#pragma unroll 4
-  for (int64_t g = i0; g < i1; g += 64) {
-    const int64_t i = g + lane;
-    const uint32_t key = i < i1 ? token_key(tokens, i, a.vocab) : a.vocab;
-    uint64_t mine = __ballot(key < a.vocab && (key & low) == me);
-    while (mine) {
-      const int first = __ffsll((unsigned long long)mine) - 1;
-      const uint32_t k = __shfl(key, first);
-      const uint64_t same = __ballot(key == k);
-      uint32_t at = 0;          // this wave's own counter of the token
-      if (lane == first) at = atomicAdd(&count[(k >> a.owner_shift) * GROUP_WAVES + wave], (uint32_t)__popcll(same));
-      at = __shfl(at, first);
-      if (key == k) {
-        const uint32_t p = at + __popcll(same & ((1ull << lane) - 1));
-        a.perm[p] = (uint32_t)i;
-        a.keys[p] = k;
+  for (int64_t g = i0; g < i1; g += 64 * AHEAD) {
+    if (i1 - i0 > 64 * AHEAD) {       // up to 16384 tokens they are still in registers
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t i = g + 64 * u + lane;
+        key[u] = i < i1 ? token_key(tokens, i, a.vocab) : a.vocab;
       }
-      mine &= ~same;
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      uint64_t mine = __ballot(key[u] < a.vocab && (key[u] & low) == me);
+      while (mine) {
+        const int first = __ffsll((unsigned long long)mine) - 1;
+        const uint32_t k = __shfl(key[u], first);
+        const uint64_t same = __ballot(key[u] == k);
+        uint32_t at = 0;          // this wave's own counter of the token
+        if (lane == first) at = atomicAdd(&count[(k >> a.owner_shift) * GROUP_WAVES + wave], (uint32_t)__popcll(same));
+        at = __shfl(at, first);
+        if (key[u] == k) {
+          const uint32_t p = at + __popcll(same & ((1ull << lane) - 1));
+          a.perm[p] = (uint32_t)(g + 64 * u + lane);
+          a.keys[p] = k;
+        }
+        mine &= ~same;
+      }
     }
   }
 }
@@ -187,6 +202,7 @@ struct SumArgs {
   const T* d_out; int64_t ldd;
   int dim;
   uint32_t vocab;
+  int64_t n;            // places there is room for
   int64_t groups;       // workgroups along the places
   int chunk, subs;      // places per chunk, chunks per workgroup
   int lane_shift;       // log2 of the lanes that share a chunk
@@ -210,9 +226,12 @@ __device__ __forceinline__ void write_row(const SumArgs<T>& a, uint32_t key, int
 
 template <int V>
 __device__ __forceinline__ void write_partial(float* dst, int left, const float (&acc)[V]) {
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    if (k < left) dst[k] = acc[k];
+  if (left >= V) store_pack<float, V>(dst, pack<float, V>(acc));
+  else store_part<float, V>(dst, pack<float, V>(acc), left);
+}
+template <int V>
+__device__ __forceinline__ void read_partial(const float* src, int left, float (&acc)[V]) {
+  unpack<float, V>(left >= V ? load_pack<float, V>(src) : load_part<float, V>(src, left), acc);
 }
 
 constexpr int MAX_CHUNK = 32, MAX_SUBS = 64;
@@ -229,14 +248,17 @@ __global__ __launch_bounds__(512) void sum_kernel(SumArgs<T> a) {
   const int64_t n = *a.placed;
   const int span = a.subs * a.chunk;
   const int64_t w0 = (int64_t)blockIdx.x * span;
+  // keys[1 + k]: place w0 + k; one more at both ends, `vocab` where the list has none.  What lies behind
+  // the n places that are taken is read (there is room) and not used: the loads need not wait for n.
+  for (int k = threadIdx.x; k < span + 2; k += threads) {
+    const int64_t p = w0 + k - 1;
+    const uint32_t key = p >= 0 && p < a.n ? a.keys[p] : a.vocab;
+    const uint32_t index = k < span && w0 + k < a.n ? a.perm[w0 + k] : 0;
+    keys[k] = p < n ? key : a.vocab;
+    if (k < span) perm[k] = index;
+  }
   if (w0 >= n) return;
   const int here = (int)(w0 + span < n ? span : n - w0);
-  // keys[1 + k]: place w0 + k; one more at both ends, `vocab` where the list has none
-  for (int k = threadIdx.x; k < here + 2; k += threads) {
-    const int64_t p = w0 + k - 1;
-    keys[k] = p >= 0 && p < n ? a.keys[p] : a.vocab;
-    if (k < here) perm[k] = a.perm[w0 + k];
-  }
   __syncthreads();
   const int p0 = sub * a.chunk, p1 = p0 + a.chunk < here ? p0 + a.chunk : here;
   if (p0 < p1 && left > 0) {
@@ -312,45 +334,48 @@ __global__ __launch_bounds__(512) void sum_kernel(SumArgs<T> a) {
 // of those it reaches, shared by the subgroups in contiguous parts.
 template <typename T>
 __global__ __launch_bounds__(512) void join_kernel(SumArgs<T> a) {
-  constexpr int V = 16 / (int)sizeof(T), AHEAD = 4;
+  constexpr int V = 16 / (int)sizeof(T), AHEAD = 8;
   extern __shared__ __attribute__((aligned(16))) float parts[];   // [threads][V]
-  const int64_t n = *a.placed;
   const int64_t span = (int64_t)a.subs * a.chunk, w0 = blockIdx.x * span, w1 = w0 + span;
-  if (w1 >= n) return;
-  const uint32_t run = a.keys[w1 - 1];
-  if (a.keys[w1] != run) return;                                       // ends here
-  if (a.keys[w0] == run && w0 > 0 && a.keys[w0 - 1] == run) return;    // began before
+  // all that decides is loaded at once: the keys around both ends of this workgroup's places, and the
+  // first keys of the next 64 workgroups
+  const int64_t n = *a.placed;
+  const int64_t next = (blockIdx.x + 1 + (int64_t)(threadIdx.x & 63)) * span;
+  const uint32_t next_key = a.keys[next < a.n ? next : 0];
+  const uint32_t before = a.keys[w0 > 0 ? w0 - 1 : 0], first = a.keys[w0];
+  const uint32_t run = a.keys[w1 - 1 < a.n ? w1 - 1 : 0], behind = a.keys[w1 < a.n ? w1 : 0];
+  if (w1 >= n || behind != run) return;                       // ends here
+  if (first == run && w0 > 0 && before == run) return;        // began before
   const int lanes = 1 << a.lane_shift;
   const int sub = threadIdx.x >> a.lane_shift, lane = threadIdx.x & (lanes - 1);
   const int c = (int)(blockIdx.y * 256 + lane) * V;
   const int left = a.dim - c < V ? a.dim - c : V;
-  // how many of the next workgroups the run reaches, 64 at a time
+  // how many of the next workgroups the run reaches
   int64_t reach = 0;
-  for (;;) {
-    const int64_t p = (blockIdx.x + 1 + reach + (threadIdx.x & 63)) * span;
-    const uint64_t other = __ballot(!(p < n && a.keys[p < n ? p : 0] == run));
-    if (other) {
-      reach += __ffsll((unsigned long long)other) - 1;
-      break;
-    }
+  uint64_t other = __ballot(!(next < n && next_key == run));
+  while (!other) {
     reach += 64;
+    const int64_t p = next + reach * span;
+    other = __ballot(!(p < n && a.keys[p < n ? p : 0] == run));
   }
+  reach += __ffsll((unsigned long long)other) - 1;
   const int64_t share = (reach + a.subs - 1) / a.subs;
   const int64_t h0 = blockIdx.x + 1 + sub * share;
   const int64_t h1 = h0 + share < blockIdx.x + 1 + reach ? h0 + share : blockIdx.x + 1 + reach;
   float acc[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = sub == 0 && k < left ? a.tail[(int64_t)blockIdx.x * a.dim + c + k] : 0.0f;
+  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+  if (sub == 0) read_partial<V>(a.tail + (int64_t)blockIdx.x * a.dim + c, left, acc);
   for (int64_t h = h0; h < h1; h += AHEAD) {
     float f[AHEAD][V];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-      for (int k = 0; k < V; ++k) f[u][k] = h + u < h1 && k < left ? a.head[(h + u) * a.dim + c + k] : 0.0f;
+      if (h + u < h1) read_partial<V>(a.head + (h + u) * a.dim + c, left, f[u]);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
+      if (h + u < h1)
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] += f[u][k];
+        for (int k = 0; k < V; ++k) acc[k] += f[u][k];
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) parts[threadIdx.x * V + k] = acc[k];
@@ -423,7 +448,7 @@ int grad_run(const void* d_out, int64_t ldd, const void* tokens, int32_t token_d
   const GradLayout l = grad_layout(n, dim, dtype);
   GroupArgs r;
   r.tokens = tokens; r.n = n; r.vocab = (uint32_t)vocab;
-  r.owners = n ? 256 : 0; r.owner_shift = 8;
+  r.owners = n ? 128 : 0; r.owner_shift = 7;    // the other CUs clear meanwhile
   while (n && (int64_t)BINS << r.owner_shift < vocab) {
     r.owners *= 2;
     ++r.owner_shift;
@@ -442,7 +467,7 @@ int grad_run(const void* d_out, int64_t ldd, const void* tokens, int32_t token_d
   if (n == 0) return PA_OK;
   SumArgs<T> a;
   a.d_out = reinterpret_cast<const T*>(d_out); a.ldd = ldd; a.dim = dim; a.vocab = (uint32_t)vocab;
-  a.groups = l.groups; a.chunk = l.chunk; a.subs = l.subs; a.lane_shift = l.lane_shift;
+  a.n = n; a.groups = l.groups; a.chunk = l.chunk; a.subs = l.subs; a.lane_shift = l.lane_shift;
   a.perm = r.perm; a.keys = r.keys; a.placed = r.placed;
   a.head = reinterpret_cast<float*>(scratch + l.head);
   a.tail = reinterpret_cast<float*>(scratch + l.tail);
