@@ -772,8 +772,8 @@ struct Split {
   int64_t tiles, chunk_tiles;
   int64_t agg_a, agg_h, agg_r, bytes;   // scratch layout
 };
-// Fewer workgroups than CUs: the steps are cut, so that there are as many workgroups as CUs (one of 16
-// waves fills a CU's registers).  The pass over the chunks' pairs is another launch and the latency of a
+// At most half as many workgroups as CUs: the steps are cut, so that there are nearly as many workgroups
+// as CUs and no more (one of 16 waves fills a CU's registers, a 257th would wait for a whole chunk).  The pass over the chunks' pairs is another launch and the latency of a
 // tile: up to three tiles are walked as they are (7 x 1001 x 257 fp16, four tiles, odd rows: forwards
 // 29 us in one piece, 23 us in four).
 Split split_of(int64_t B, int64_t T, int D, bool grad) {
@@ -782,7 +782,7 @@ Split split_of(int64_t B, int64_t T, int D, bool grad) {
   s.slabs = (int)ceil_div(D, brief ? Short::SLAB : middle ? Middle::SLAB : Long::SLAB);
   s.tiles = ceil_div(T, brief ? Short::STEPS : middle ? Middle::STEPS : grad ? LongGrad::STEPS : Long::STEPS);
   const int64_t groups = B * s.slabs;
-  int64_t chunks = groups >= 192 || s.tiles <= 3 ? 1 : ceil_div(256, groups);
+  int64_t chunks = groups > 128 || s.tiles <= 3 ? 1 : 256 / groups;
   if (chunks > s.tiles) chunks = s.tiles;
   s.chunk_tiles = ceil_div(s.tiles, chunks);
   s.chunks = (int)ceil_div(s.tiles, s.chunk_tiles);
