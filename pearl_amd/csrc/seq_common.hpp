@@ -25,6 +25,7 @@ class DeviceGuard {
     }
     if (e != hipSuccess) {
       set_error("device %d: %s", device, hipGetErrorString(e));
+      (void)hipGetLastError();      // or the caller's next call would report it
       rc_ = PA_ERR_HIP;
     }
   }

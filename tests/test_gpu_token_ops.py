@@ -69,7 +69,8 @@ def test_embed_tokens_outside_the_table_and_strided(dtype):
 @pytest.mark.parametrize("n,vocab,dim,kind", [(1, 1, 1, "any"), (1, 300, 5, "any"), (7, 4, 3, "any"),
                                               (64, 1, 17, "same"), (65, 9, 130, "any"), (700, 30, 333, "skew"),
                                               (1500, 5000, 40, "any"), (2100, 3, 2050, "same"), (4099, 700, 24, "skew"),
-                                              (9000, 17, 12, "none")])
+                                              (9000, 17, 12, "none"),
+                                              (20000, 70000, 6, "skew"), (40000, 5, 3, "same")])
 def test_embed_grad(dtype, n, vocab, dim, kind):
     from pearl_amd import embed_tokens_grad
     gen = gen_of(n, vocab, dim, 1)
@@ -85,6 +86,7 @@ def test_embed_grad(dtype, n, vocab, dim, kind):
         tok[::97] = vocab + 5
         tok[::89] = -7
     d = rnd(gen, n, dim, dtype=dtype)
+    d[((tok < 0) | (tok >= vocab)).to(DEV)] = float("nan")        # rows without a token take no part
     value, bound = O.embed_grad(np64(d), tok.numpy(), vocab, 1.7)
     for index in (torch.int64, torch.int32):
         got = embed_tokens_grad(d, tok.to(DEV, index), vocab, scale=1.7)
@@ -152,7 +154,7 @@ def check_recurrence(c, logits, reverse, dtype, gate_dtype, what=""):
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("logits", [True, False], ids=["logit", "decay"])
 @pytest.mark.parametrize("b,t,d", [(1, 1, 1), (3, 1, 70), (2, 2, 5), (2, 31, 64), (2, 32, 65), (3, 33, 9), (1, 257, 40),
-                                   (2, 300, 129), (1, 1500, 17)])
+                                   (2, 300, 129), (1, 1500, 17), (2, 128, 40), (1, 129, 33), (1, 256, 2), (2, 1030, 66)])
 def test_gated_recurrence(dtype, logits, b, t, d):
     for k, (reverse, resets, lengths) in enumerate([(False, False, False), (True, True, False), (False, True, True),
                                                     (True, False, True)]):
@@ -188,6 +190,10 @@ def test_gated_recurrence_strided_inputs():
     check_recurrence(c, True, False, torch.bfloat16, torch.bfloat16, "one gate: ")
     c["x"] = rnd(gen, 2, 37, 70, dtype=torch.bfloat16).transpose(1, 2)     # channels not adjacent
     check_recurrence(c, True, False, torch.bfloat16, torch.bfloat16, "channels: ")
+    far = torch.zeros(70, 2 ** 22 + 5, dtype=torch.bfloat16, device=DEV)[:, :37]     # steps 8 MB apart
+    far.copy_(rnd(gen, 70, 37, dtype=torch.bfloat16))
+    c["x"] = far.unsqueeze(0).expand(2, 70, 37)
+    check_recurrence(c, True, True, torch.bfloat16, torch.bfloat16, "far: ")
 
 
 def test_gated_recurrence_resets_forget_and_padding_hides_anything():
@@ -535,3 +541,84 @@ def test_operators_in_two_graphs_replayed_with_new_inputs():
         torch.cuda.synchronize()
         for got, w in zip(outs, want):
             assert all(torch.equal(x, y) for x, y in zip(got, w)), k
+
+
+def test_acting_step_in_a_graph_advances_its_state_in_place():
+    from pearl_amd import gated_recurrence, gated_recurrence_step
+    gen = gen_of(61)
+    xs, gs = rnd(gen, 3, 6, 21, dtype=torch.bfloat16), rnd(gen, 3, 6, 21, dtype=torch.bfloat16)
+    x, g, state = xs[:, 0].clone(), gs[:, 0].clone(), torch.zeros(3, 21, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gated_recurrence_step(x, g, state)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, _ = gated_recurrence_step(x, g, state, out_state=state)
+    state.zero_()
+    want, last = gated_recurrence(xs, gs)
+    for t in range(6):
+        x.copy_(xs[:, t])
+        g.copy_(gs[:, t])
+        graph.replay()
+        torch.testing.assert_close(h.float(), want[:, t].float(), rtol=2.0 ** -7, atol=2.0 ** -14)
+    torch.testing.assert_close(state, last, rtol=0, atol=100 * O.U * float(last.abs().max()))
+
+
+def test_unknown_device_is_refused():
+    from pearl_amd import _native as N
+    w, tok, out = torch.randn(4, 4, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV), torch.empty(2, 4, device=DEV)
+    rc = N.lib().pa_embed_tokens(w.data_ptr(), N.PA_F32, 4, 4, 4, tok.data_ptr(), N.PA_I64, 2, 1.0, out.data_ptr(), 1000, None)
+    assert rc == N.PA_ERR_HIP and "1000" in N.last_error()
+    assert torch.cuda.current_device() == 0
+
+
+# ---------------------------------------------------------------------------- offsets behind 2^31 elements
+def test_embed_tokens_behind_two_to_the_31st_element():
+    from pearl_amd import embed_tokens, embed_tokens_grad
+    vocab, dim = 2 ** 21 + 77, 1030
+    w = torch.zeros(vocab, dim, dtype=torch.bfloat16, device=DEV)
+    w[-3:] = torch.arange(3 * dim, device=DEV).view(3, dim).remainder(251).to(torch.bfloat16)
+    tok = torch.tensor([vocab - 1, 0, vocab - 3, vocab - 1], device=DEV)
+    out = embed_tokens(w, tok)
+    assert torch.equal(out, w[tok]) and out[0].abs().sum() > 0
+    d = torch.ones(4, dim, dtype=torch.bfloat16, device=DEV)
+    dw = embed_tokens_grad(d, tok, vocab)
+    assert (dw[-1] == 2).all() and (dw[-2] == 0).all() and (dw[-3] == 1).all() and (dw[0] == 1).all()
+    assert float(dw[1:-3].abs().max()) == 0
+
+
+def test_gated_recurrence_behind_two_to_the_31st_element():
+    from pearl_amd import gated_recurrence, gated_recurrence_grad
+    t, d = 2 ** 21 + 1000, 1030
+    x = torch.empty(1, t, d, dtype=torch.bfloat16, device=DEV).normal_()
+    g = torch.empty(1, t, d, dtype=torch.bfloat16, device=DEV).normal_()
+    h, last, kept = gated_recurrence(x, g, keep=True)
+    cut = t - 500
+    _, middle = gated_recurrence(x[:, cut - 2000:cut], g[:, cut - 2000:cut])     # gates near 1/2: far states do not matter
+    h2, last2, kept2 = gated_recurrence(x[:, cut:], g[:, cut:], middle, keep=True)
+    torch.testing.assert_close(last, last2, rtol=0, atol=200 * O.U * 4)
+    torch.testing.assert_close(h[:, cut:].float(), h2.float(), rtol=2.0 ** -7, atol=2.0 ** -12)
+    d_h = torch.empty(1, t, d, dtype=torch.bfloat16, device=DEV).normal_()
+    a = gated_recurrence_grad(x, g, kept, d_h)
+    b = gated_recurrence_grad(x[:, cut:], g[:, cut:], kept2, d_h[:, cut:])
+    for k in (0, 1):
+        torch.testing.assert_close(a[k][:, cut:].float(), b[k].float(), rtol=2.0 ** -7, atol=2.0 ** -10)
+
+
+def test_action_log_probs_behind_two_to_the_31st_element():
+    from pearl_amd import action_log_probs, action_log_probs_grad
+    rows, width = 66000, 32771
+    logits = torch.empty(rows, width, dtype=torch.bfloat16, device=DEV).normal_()
+    actions = torch.randint(0, width, (rows,), device=DEV)
+    o = action_log_probs(logits, actions, top=3)
+    few = action_log_probs(logits[-600:], actions[-600:], top=3)
+    assert torch.equal(o.log_prob[-600:], few.log_prob) and torch.equal(o.entropy[-600:], few.entropy)
+    assert torch.equal(o.top_actions[-600:], few.top_actions)
+    g_lp, g_h = torch.randn(rows, device=DEV), torch.randn(rows, device=DEV)
+    d = action_log_probs_grad(o, logits, actions, g_lp, g_h)
+    assert torch.equal(d[-600:], action_log_probs_grad(few, logits[-600:], actions[-600:], g_lp[-600:], g_h[-600:]))
+    want = O.log_probs(np64(logits[-2:]), actions[-2:].cpu().numpy(), None, 1.0, 3, np64(g_lp[-2:]), np64(g_h[-2:]))
+    O.check(o.log_prob[-2:], *want["log_prob"], torch.float32, "log_prob")
+    O.check(d[-2:], *want["d_logits"], torch.bfloat16, "d_logits")

@@ -43,6 +43,7 @@ def test_c_entries_refuse_bad_arguments():
         assert embed(**bad) == N.PA_ERR_INVALID, bad
     grad = lambda dtype=N.PA_BF16, n=2, vocab=8, dim=4, tdt=N.PA_I32, d=buf, t=buf, w=buf, s=buf, ldd=4: lib.pa_embed_tokens_grad(  # noqa: E731
         d, dtype, ldd, t, tdt, n, 1.0, vocab, dim, w, s, 0, None)
+    assert grad(n=2 ** 26 + 1) == grad(vocab=2 ** 26 + 1) == N.PA_ERR_UNSUPPORTED
     assert grad(dtype=N.PA_I64) == grad(tdt=N.PA_F32) == N.PA_ERR_UNSUPPORTED
     for bad in (dict(dim=0), dict(vocab=0), dict(n=-1), dict(d=None), dict(t=None), dict(w=None), dict(s=None), dict(ldd=-1)):
         assert grad(**bad) == N.PA_ERR_INVALID, bad
@@ -57,6 +58,8 @@ def test_c_entries_refuse_bad_arguments():
         return (lib.pa_gated_recurrence_grad if grad else lib.pa_gated_recurrence)(C.byref(a), None)
     assert rec(B=0) == rec(True, B=0) == N.PA_OK
     assert rec(dtype=N.PA_I64) == rec(gate_dtype=N.PA_F16) == rec(dtype=N.PA_F32) == N.PA_ERR_UNSUPPORTED
+    for far in (dict(x_t=2 ** 22), dict(gate_t=2 ** 22), dict(resets_t=2 ** 23), dict(d_h_t=2 ** 22), dict(x_t=-1), dict(D=2 ** 21)):
+        assert rec(**far) == N.PA_ERR_UNSUPPORTED, far
     for bad in (dict(T=0), dict(D=0), dict(B=-1), dict(x=None), dict(gate=None), dict(h=None), dict(B=2 ** 40),
                 dict(B=1, T=4000, scratch=None)):
         assert rec(**bad) == N.PA_ERR_INVALID, bad
