@@ -44,12 +44,16 @@ struct LpArgs {
   T* d_logits;                             // [rows][A]
 };
 
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
+
 // m, s, u of some of a row's elements, in units of the logits; empty: m = -inf, s = u = 0
 struct Sums {
   float m, s, u;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) { return (a != a || b != b) ? __builtin_nanf("") : fmaxf(a, b); }
 
 // brings the sums in front of a new maximum
 __device__ __forceinline__ void move_to(Sums& x, float m, float c) {
@@ -61,13 +65,23 @@ __device__ __forceinline__ void move_to(Sums& x, float m, float c) {
   x.m = m;
 }
 __device__ __forceinline__ Sums join(Sums x, Sums y, float c) {
-  const float m = max_nan(x.m, y.m);
+  const float m = __builtin_elementwise_maximum(x.m, y.m);
   move_to(x, m, c);
   move_to(y, m, c);
   return {m, x.s + y.s, x.u + y.u};
 }
-__device__ __forceinline__ Sums shuffle_xor(const Sums& x, int o) {
-  return {__shfl_xor(x.m, o), __shfl_xor(x.s, o), __shfl_xor(x.u, o)};
+// of all lanes of a wave: the maximum first, so that every lane moves its sums once
+__device__ __forceinline__ Sums join_lanes(Sums x, float c) {
+  float m = x.m;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o));
+  move_to(x, m, c);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    x.s += __shfl_xor(x.s, o);
+    x.u += __shfl_xor(x.u, o);
+  }
+  return x;
 }
 // the elements' maximum must be taken first: e <= 1.  An element below the maximum by more than the
 // range of a float, -inf among them, adds nothing.
@@ -75,6 +89,26 @@ __device__ __forceinline__ void add_to(Sums& x, float v, float c) {
   const float d = fmaxf(v - x.m, -FLT_MAX), e = __builtin_amdgcn_exp2f(d * c);
   x.s += e;
   x.u = fmaf(e, d, x.u);
+}
+
+// The same for N elements at once without the clamp, which costs an instruction an element: an -inf among
+// them turns the second sum into NaN, and the elements are added again with it.
+template <int N>
+__device__ __forceinline__ void add_all(Sums& x, const float (&v)[N], float c) {
+  float s = x.s, u = x.u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = v[i] - x.m, e = __builtin_amdgcn_exp2f(d * c);
+    s += e;
+    u = fmaf(e, d, u);
+  }
+  if (u == u) {
+    x.s = s;
+    x.u = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) add_to(x, v[i], c);
+  }
 }
 
 // order of the alternatives: larger logits first, then lower index; NaN ranks above all.  0: none.
@@ -179,8 +213,8 @@ __global__ __launch_bounds__(256) void small_kernel(LpArgs<T> a) {
     const int64_t row = on ? mine : a.rows - 1;     // every lane takes part in the shuffles
     float f[4];
     load_four(a, row, lane * 4, f);
-    Sums x = {max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3])), 0.0f, 0.0f};
-    for (int o = 1; o < lanes; o *= 2) x.m = max_nan(x.m, __shfl_xor(x.m, o));
+    Sums x = {__builtin_elementwise_maximum(__builtin_elementwise_maximum(f[0], f[1]), __builtin_elementwise_maximum(f[2], f[3])), 0.0f, 0.0f};
+    for (int o = 1; o < lanes; o *= 2) x.m = __builtin_elementwise_maximum(x.m, __shfl_xor(x.m, o));
 #pragma unroll
     for (int i = 0; i < 4; ++i) add_to(x, f[i], c);
     for (int o = 1; o < lanes; o *= 2) {
@@ -246,6 +280,28 @@ struct Best {
   }
 };
 
+// What a lane reads at once: U packs of logits and their mask bytes.  A pack that would pass the end of
+// the row is moved back to end with it, so that all are whole; what is not of this place is left out later.
+template <typename T, int U>
+struct Batch {
+  static constexpr int V = 16 / (int)sizeof(T);
+  Pack<T, V> p[U];
+  uint32_t m[U][V / 4];
+};
+template <typename T, int U>
+__device__ __forceinline__ void load_batch(Batch<T, U>& r, const T* src, const uint8_t* msk, int64_t j0, int step, int A) {
+  constexpr int V = Batch<T, U>::V;
+  typedef uint32_t B __attribute__((aligned(1), may_alias));
+#pragma unroll
+  for (int q = 0; q < U; ++q) {
+    const int64_t j = j0 + (int64_t)q * step, at = j < A - V ? j : A - V;
+    r.p[q] = load_pack<T, V>(src + at);
+    if (msk)
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) r.m[q][k] = reinterpret_cast<const B*>(msk + at)[k];
+  }
+}
+
 // W waves share a row's piece; 4 / W pieces per workgroup
 template <typename T, int W, bool TOP>
 __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
@@ -253,7 +309,7 @@ __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
   constexpr int STEP = W * 64 * V;
   __shared__ Sums sums[4];
   __shared__ uint64_t lists[TOP ? 4 : 1][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part_wave = wave & (W - 1);
   const float c = a.inv_t * LOG2E;
   const int64_t pieces = a.rows * a.chunks;
@@ -269,36 +325,43 @@ __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
     uint64_t least = 0;            // the key that a new alternative has to pass
     float least_value = -INFINITY;
     bool seeded = false;
-    for (int64_t base = ch * a.chunk + (int64_t)part_wave * 64 * V; base < j1; base += (int64_t)STEP * U) {
+    int64_t base = ch * a.chunk + (int64_t)part_wave * 64 * V;
+    constexpr int64_t BATCH = (int64_t)STEP * U;
+    const auto sum_up = [&](const Batch<T, U>& cur) {
       float f[U][V];
 #pragma unroll
-      for (int q = 0; q < U; ++q) {
-        const int64_t j = base + (int64_t)q * STEP + lane * V;
-        const int64_t left = j1 - j;
-        if (left >= V) {
-          unpack<T, V>(load_pack<T, V>(src + j), f[q]);
-          if (msk) apply_mask_full<V>(f[q], msk + j);
-        } else {
+      for (int q = 0; q < U; ++q) unpack<T, V>(cur.p[q], f[q]);
+      if (msk) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[q][i] = i < left ? (float)src[j + i] : -INFINITY;
-          if (msk) apply_mask<V>(f[q], msk + j, left > 0 ? (int)left : 0);
+        for (int q = 0; q < U; ++q)
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if ((cur.m[q][i / 4] >> (8 * (i & 3))) & 0xff) f[q][i] = -INFINITY;
+      }
+      if (base + (int64_t)(U - 1) * STEP + 64 * V > j1) {       // some of the packs pass the end of the piece
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+          const int64_t j = base + (int64_t)q * STEP + lane * V, at = j < a.A - V ? j : a.A - V;
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (at + i < j || at + i >= j1) f[q][i] = -INFINITY;
         }
       }
-      float bm = -INFINITY;
-      bool nan = false;
+      float bm = f[0][0];      // maximum, not fmax: a NaN stays
 #pragma unroll
       for (int q = 0; q < U; ++q)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          bm = fmaxf(bm, f[q][i]);
-          nan = nan || f[q][i] != f[q][i];
-        }
-      if (nan) bm = __builtin_nanf("");
+        for (int i = 0; i < V; ++i) bm = __builtin_elementwise_maximum(bm, f[q][i]);
       if (!(bm <= x.m) && x.m == x.m) move_to(x, bm, c);
+      if (msk) {
 #pragma unroll
-      for (int q = 0; q < U; ++q)
+        for (int q = 0; q < U; ++q)
 #pragma unroll
-        for (int i = 0; i < V; ++i) add_to(x, f[q][i], c);
+          for (int i = 0; i < V; ++i) add_to(x, f[q][i], c);
+      } else {
+#pragma unroll
+        for (int q = 0; q < U; ++q) add_all<V>(x, f[q], c);
+      }
 
       if constexpr (TOP) {
         uint64_t skip = 0;
@@ -308,7 +371,8 @@ __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
           for (int q = 0; q < U; ++q)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const uint64_t k = key_of(f[q][i], (uint32_t)(base + (int64_t)q * STEP + lane * V + i));
+              const int64_t j = base + (int64_t)q * STEP + lane * V, at = j < a.A - V ? j : a.A - V;
+              const uint64_t k = key_of(f[q][i], (uint32_t)(at + i));
               skip = k > skip ? k : skip;
             }
           best.key = skip;
@@ -330,8 +394,8 @@ __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
             if (cand) {
               const int e = __ffs(cand) - 1;
               cand &= cand - 1;
-              const int64_t j = base + (int64_t)(e / V) * STEP + lane * V + e % V;
-              k = key_of((float)src[j], (uint32_t)j);
+              const int64_t j = base + (int64_t)(e / V) * STEP + lane * V, at = (j < a.A - V ? j : a.A - V) + e % V;
+              k = key_of((float)src[at], (uint32_t)at);
               if (k == skip) k = 0;
             }
             uint64_t todo = __ballot(k > least);
@@ -346,9 +410,20 @@ __global__ __launch_bounds__(256) void large_kernel(LpArgs<T> a) {
           least_value = value_of(least);
         }
       }
+    };
+    // two batches in turn: while one is summed the next is under way, and none is copied
+    Batch<T, U> even, odd;
+    if (base < j1) load_batch(even, src, msk, base + lane * V, STEP, a.A);
+    while (base < j1) {
+      if (base + BATCH < j1) load_batch(odd, src, msk, base + BATCH + lane * V, STEP, a.A);
+      sum_up(even);
+      base += BATCH;
+      if (base >= j1) break;
+      if (base + BATCH < j1) load_batch(even, src, msk, base + BATCH + lane * V, STEP, a.A);
+      sum_up(odd);
+      base += BATCH;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = join(x, shuffle_xor(x, o), c);
+    x = join_lanes(x, c);
     if constexpr (W > 1) {
       if (lane == 0) sums[wave] = x;
       if constexpr (TOP) lists[wave][lane] = best.key;
@@ -405,8 +480,7 @@ __global__ __launch_bounds__(256) void finish_kernel(LpArgs<T> a) {
     const float* p = a.part + 3 * (row * a.chunks + ch);
     x = join(x, Sums{p[0], p[1], p[2]}, c);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) x = join(x, shuffle_xor(x, o), c);
+  x = join_lanes(x, c);
   float log_s = 0.0f;
   if (lane == 0) finish_row(a, row, x, log_s);
   if constexpr (TOP) {
@@ -444,22 +518,27 @@ __device__ __forceinline__ RowGrad row_grad(const LpArgs<T>& a, int64_t row) {
   }
   return r;
 }
-// f: logits in (-inf: unavailable), gradients out
-template <int N>
+// f: logits in (-inf: unavailable), gradients out.  With the row's constants gathered,
+//   dl = p (k0 + k1 log2 p),  k0 = -(g_lp + g_H H) / T,  k1 = -g_H ln 2 / T.
+// CHECK: the row is not an ordinary one (no action left, or NaN, which must not reach unavailable places).
+template <int N, bool CHECK>
 __device__ __forceinline__ void grad_of(float (&f)[N], int64_t j, const RowGrad& r, float c, float inv_t) {
+  const float k0 = -fmaf(r.g_h, r.h, r.g_lp) * inv_t, k1 = -r.g_h * LN2 * inv_t;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     // the clamp keeps p log p at zero where p has underflowed
-    const float t2 = fmaxf((f[i] - r.m) * c - r.log2s, -1.0e4f);
-    const float p = __builtin_amdgcn_exp2f(t2);
-    const float d = -p * (r.g_lp + r.g_h * fmaf(t2, LN2, r.h));
-    f[i] = (f[i] == -INFINITY || r.none) ? 0.0f : d * inv_t;
+    const float t2 = fmaxf(fmaf(f[i] - r.m, c, -r.log2s), -1.0e4f);
+    const float d = __builtin_amdgcn_exp2f(t2) * fmaf(k1, t2, k0);
+    f[i] = CHECK && (f[i] == -INFINITY || r.none) ? 0.0f : d;
   }
   if (r.t >= j && r.t < j + N) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (j + i == r.t) f[i] += r.g_lp * inv_t;
+      if (j + i == r.t) f[i] = fmaf(r.g_lp, inv_t, f[i]);
   }
+}
+__device__ __forceinline__ bool ordinary(const RowGrad& r) {
+  return r.m > -INFINITY && r.m < INFINITY && r.h == r.h && r.g_lp == r.g_lp && r.g_h == r.g_h;
 }
 
 template <typename T>
@@ -472,7 +551,7 @@ __global__ __launch_bounds__(256) void small_grad_kernel(LpArgs<T> a) {
     const RowGrad r = row_grad(a, row);
     float f[4];
     load_four(a, row, j, f);
-    grad_of<4>(f, j, r, c, a.inv_t);
+    grad_of<4, true>(f, j, r, c, a.inv_t);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (j + i < a.A) a.d_logits[row * a.A + j + i] = (T)f[i];
@@ -487,26 +566,29 @@ __global__ __launch_bounds__(256) void large_grad_kernel(LpArgs<T> a) {
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
     const int64_t row = piece / per_row;
     const int64_t base = (piece - row * per_row) * STEP * U + threadIdx.x * V;
-    const RowGrad r = row_grad(a, row);
     const T* src = a.logits + row * a.ld;
     const uint8_t* msk = a.mask ? a.mask + row * a.ldm : nullptr;
     T* dst = a.d_logits + row * a.A;
+    Batch<T, U> in;                     // a row's last pack is moved back; its places are written twice, alike
+    load_batch(in, src, msk, base, STEP, a.A);
+    const RowGrad r = row_grad(a, row);
+    const auto write = [&](auto checked) {
 #pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int64_t j = base + q * STEP, left = a.A - j;
-      float f[V];
-      if (left >= V) {
-        unpack<T, V>(load_pack<T, V>(src + j), f);
-        if (msk) apply_mask_full<V>(f, msk + j);
-        grad_of<V>(f, j, r, c, a.inv_t);
-        store_pack<T, V>(dst + j, pack<T, V>(f));
-      } else if (left > 0) {
-        unpack<T, V>(load_part<T, V>(src + j, (int)left), f);
-        if (msk) apply_mask<V>(f, msk + j, (int)left);
-        grad_of<V>(f, j, r, c, a.inv_t);
-        store_part<T, V>(dst + j, pack<T, V>(f), (int)left);
+      for (int q = 0; q < U; ++q) {
+        const int64_t j = base + q * STEP, at = j < a.A - V ? j : a.A - V;
+        float f[V];
+        unpack<T, V>(in.p[q], f);
+        if (msk) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if ((in.m[q][i / 4] >> (8 * (i & 3))) & 0xff) f[i] = -INFINITY;
+        }
+        grad_of<V, decltype(checked)::value>(f, at, r, c, a.inv_t);
+        if (j < a.A) store_pack<T, V>(dst + at, pack<T, V>(f));
       }
-    }
+    };
+    if (ordinary(r)) write(Bool<false>());
+    else write(Bool<true>());
   }
 }
 
