@@ -8,15 +8,21 @@
 // scanned in parallel.  A reset makes its step ignore the state before it: not a factor of zero (zero
 // times infinity is not zero) but a flag that travels with the pair and selects.
 //
-// A workgroup owns a slab of channels that is one 128-byte line wide in the input's type and walks the
-// steps in tiles: 8 lanes side by side in a row of x, 8 groups of L consecutive steps per wave, waves
-// behind one another in time.  Each lane scans its own L steps, groups are joined by lane shuffles,
-// waves through LDS, the state behind the tile stays in LDS for the next one while that tile's loads
-// are already under way.  Every input is read once and every output written once.  The state is fp32
-// throughout; only the stored h is rounded to the input's type.
+// A workgroup owns a slab of 64 channels (a 128-byte line of 16-bit values) and walks the steps in tiles:
+// 32 lanes of two channels side by side in a row, two groups of 8 consecutive steps per wave, waves behind
+// one another in time.  Each lane scans its own steps, the groups are joined by one lane shuffle, the
+// waves through LDS by one wave, which carries the state on, while the next tile's loads are already under
+// way.  Every input is read once and every output written once.  The state is fp32 throughout; only the
+// stored h is rounded to the input's type.
+//
+// Two channels a lane, because what a step costs beside its loads is the joining: with eight a lane (16-byte
+// loads) the tile needs three shuffles of 16 values (61 us against 49 at 16 x 2048 x 1024 bf16, 201 MB; the
+// same accesses without arithmetic take 31).  Forwards 21 VALU instructions a value, backwards 40; the rest
+// of the time is the tile's two barriers.
 //
 // Where batch x channels give too few workgroups, the steps are cut into chunks: a first launch
-// composes each chunk's pair, the second starts every chunk from the composition of those before it.
+// composes each chunk's pair, the second starts every chunk from the composition of those before it
+// (1 x 65536 x 512 bf16: 32 + 42 us; the inputs are read twice).
 //
 // Backward, with G_t = dh_t + c_t and c_{t-1} = a_t G_t (0 at a reset), c_T = d_last:
 //   decay:  dx = G, dg = G h_{t-1};   logit:  dx = (1 - a) G, dg = a (1 - a) G (h_{t-1} - x);
@@ -36,9 +42,9 @@ struct Shape {
   static constexpr int NW = NW_, CL = CL_, L = L_, V = V_, TG = 64 / CL_, STEPS = NW_ * TG * L_, SLAB = CL_ * V_;
 };
 typedef Shape<1, 16, 8, 2> Short;          // histories of up to 32 steps
-typedef Shape<8, 16, 4, 2> Middle;         // of up to 128
+typedef Shape<8, 16, 4, 2> Middle;         // of up to 128: half-width slabs (1 x 128 x 4096 fp32 6.2 us; as Long 14.4)
 typedef Shape<16, 32, 8, 2> Long;          // longer ones, forwards
-typedef Shape<8, 32, 8, 2> LongGrad;       // longer ones, backwards
+typedef Shape<8, 32, 8, 2> LongGrad;       // longer ones, backwards: 16 waves of 8 steps would spill (240 us, not 91)
 constexpr int KEEP = Long::STEPS / LongGrad::STEPS;
 static_assert(Short::SLAB <= 64 && Middle::SLAB <= 64 && Long::SLAB <= 64 && LongGrad::SLAB == Long::SLAB,
               "a lane of a wave carries the state of each channel");
