@@ -412,6 +412,11 @@ GradLayout grad_layout(int64_t n, int dim, int dtype) {
   while ((l.subs << l.lane_shift) < 64) l.subs *= 2;
   while ((l.subs << l.lane_shift) > 512) l.subs /= 2;
   l.chunk = 2;
+  if (n <= (int64_t)l.subs * MAX_CHUNK && n * dim * elem_size(dtype) <= 16 * 1024) {
+    // so little that one workgroup sums it all, which saves the launch that joins (50 x 128 bf16, a call with
+    // its lookup: 20.4 us, in many workgroups 23.1; 256 x 100: 30.5 and 22.9)
+    while (n > (int64_t)l.chunk * l.subs) l.chunk *= 2;
+  }
   while (l.chunk < MAX_CHUNK && n > (int64_t)l.chunk * l.subs * 256) l.chunk *= 2;
   l.groups = ceil_div(n, (int64_t)l.chunk * l.subs);
   l.placed = 0;

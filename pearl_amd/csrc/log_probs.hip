@@ -596,6 +596,11 @@ __global__ __launch_bounds__(256) void large_grad_kernel(LpArgs<T> a) {
   }
 }
 
+// A row of up to this many batches of four waves is not cut: the launch that joins costs more than the
+// batches do one after another (3 x 31698 bf16, a call: 12.9 us whole, 17.0 in four pieces; 300 rows with 20
+// alternatives 23 and 33; 3 rows with 20 alternatives 21.2 and 19.9).
+constexpr int WHOLE = 4;
+
 // pieces of a row: few rows are cut so that the card is filled (16 x 131072 bf16 with 20 alternatives: 12.3
 // us in 256 pieces and 6 us to join them; a row is 16 batches of a workgroup, about 2 us each, in one piece)
 struct Pieces {
@@ -604,8 +609,8 @@ struct Pieces {
 };
 Pieces pieces_of(int64_t rows, int64_t A, int dtype, int top) {
   Pieces p = {1, A, 0, 0};
-  if (A > SMALL && rows < 512) {
-    const int64_t step = 4 * 256 * 16 / elem_size(dtype);    // what four waves read at once
+  const int64_t step = 4 * 256 * 16 / elem_size(dtype);    // what four waves read at once
+  if (A > WHOLE * step && rows < 512) {
     int64_t chunks = ceil_div(1024, rows > 0 ? rows : 1);
     if (chunks > ceil_div(A, step)) chunks = ceil_div(A, step);
     if (chunks > 128) chunks = 128;

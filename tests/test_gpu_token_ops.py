@@ -96,6 +96,15 @@ def test_embed_grad(dtype, n, vocab, dim, kind):
     assert torch.equal(got, again)
 
 
+def test_embed_grad_without_tokens_clears_the_table():
+    from pearl_amd import embed_tokens_grad
+    for dtype in DTYPES:
+        d = embed_tokens_grad(torch.empty(0, 5, dtype=dtype, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV), 7)
+        assert d.shape == (7, 5) and d.dtype == dtype and (d == 0).all()
+        none = torch.full((3,), -1, device=DEV)
+        assert (embed_tokens_grad(torch.full((3, 5), float("nan"), dtype=dtype, device=DEV), none, 7) == 0).all()
+
+
 def test_embed_grad_strided_and_broadcast_gradients():
     from pearl_amd import embed_tokens, embed_tokens_grad
     gen = gen_of(11)
@@ -515,7 +524,7 @@ def test_operators_on_two_streams_at_once():
 
 
 def test_operators_in_two_graphs_replayed_with_new_inputs():
-    few = dict(b=1, t=900, d=24, vocab=100, width=9000)
+    few = dict(b=1, t=400, d=24, vocab=100, width=20000)      # cut histories and rows: scratch in both graphs
     statics = [a_state(0, **few), a_state(1, **few)]
     a_run(statics[0])
     torch.cuda.synchronize()
