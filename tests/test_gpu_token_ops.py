@@ -524,7 +524,7 @@ def test_operators_on_two_streams_at_once():
 
 
 def test_operators_in_two_graphs_replayed_with_new_inputs():
-    few = dict(b=1, t=400, d=24, vocab=100, width=20000)      # cut histories and rows: scratch in both graphs
+    few = dict(b=1, t=900, d=24, vocab=100, width=20000)      # cut histories and rows: scratch in both graphs
     statics = [a_state(0, **few), a_state(1, **few)]
     a_run(statics[0])
     torch.cuda.synchronize()
