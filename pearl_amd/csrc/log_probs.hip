@@ -177,25 +177,6 @@ __device__ __forceinline__ void write_top(const LpArgs<T>& a, int64_t row, int k
   a.top_log_probs[row * a.top + k] = key ? (value_of(key) - x.m) * a.inv_t - log_s : -INFINITY;
 }
 
-template <int N>
-__device__ __forceinline__ void apply_mask(float (&f)[N], const uint8_t* m, int left) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < left && m[i]) f[i] = -INFINITY;
-}
-// N mask bytes as words, at byte alignment
-template <int N>
-__device__ __forceinline__ void apply_mask_full(float (&f)[N], const uint8_t* m) {
-  typedef uint32_t U __attribute__((aligned(1), may_alias));
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const uint32_t w = *reinterpret_cast<const U*>(m + i);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if ((w >> (8 * k)) & 0xff) f[i + k] = -INFINITY;
-  }
-}
-
 // ---- up to 256 actions: a few lanes per row, four actions per lane, all in registers ---------------
 // (65536 x 16 fp32 with masks: 5.3 us forwards, 6.2 backwards, 17 MB in all)
 constexpr int SMALL = 256;
