@@ -68,10 +68,10 @@ struct RecArgs {
   T* dx; G* dg; float* dh0;                      // dh0 or null
 };
 
-// a and 1 - a of a logit, both to a few ulp, also where one of them is tiny.  Below -80 a stays at 2e-35
-// (exp would overflow); NaN stays NaN (maximum, not fmax).
+// a and 1 - a of a logit, both to a few ulp, also where one of them is tiny.  Below -87 a stays at 2e-38,
+// the smallest normal number (1 / a would overflow); NaN stays NaN (maximum, not fmax).
 __device__ __forceinline__ float exp_minus(float z) {
-  return __builtin_amdgcn_exp2f(-1.44269504088896340736f * __builtin_elementwise_maximum(z, -80.0f));
+  return __builtin_amdgcn_exp2f(-1.44269504088896340736f * __builtin_elementwise_maximum(z, -87.0f));
 }
 __device__ __forceinline__ void gate_of(float e, float& a, float& keep) {
   a = __builtin_amdgcn_rcpf(1.0f + e);

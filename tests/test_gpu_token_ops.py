@@ -234,6 +234,34 @@ def test_gated_recurrence_resets_forget_and_padding_hides_anything():
                 assert (h2[i, e:] == 0).all() and (g2[0][i, e:] == 0).all() and (g2[1][i, e:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_gated_recurrence_saturated_gates(dtype):
+    """Gates far out, infinite among them: the state is kept or replaced, nothing turns into NaN."""
+    from pearl_amd import gated_recurrence, gated_recurrence_grad
+    inf = float("inf")
+    x = rnd(gen_of(71), 1, 8, 20, dtype=dtype)
+    h0 = rnd(gen_of(72), 1, 20)
+    g = torch.tensor([200.0, inf, -200.0, 1e4, inf, -inf, 87.5, -87.5], device=DEV).to(dtype).view(1, 8, 1).expand(1, 8, 20)
+    h, last, kept = gated_recurrence(x, g, h0, keep=True)
+    want = torch.stack([h0, h0, x[:, 2].float(), x[:, 2].float(), x[:, 2].float(), x[:, 5].float(), x[:, 5].float(), x[:, 7].float()], 1)
+    assert float((last - want[:, -1]).abs().max()) < 1e-30
+    assert torch.equal(h.float(), want.to(dtype).float())
+    d = rnd(gen_of(73), 1, 8, 20, dtype=dtype)
+    dx, dg, d0 = gated_recurrence_grad(x, g, kept, d)
+    assert float(dg.float().abs().max()) < 1e-30
+    torch.testing.assert_close(d0, (d[:, 0].float() + d[:, 1].float()), rtol=4 * O.U, atol=0)
+    # a sum of three in fp32 is off by at most 2 U times the sum of their sizes in either order, so two orders
+    # differ by 4 U of it, and by one rounding to the type each
+    three = d[:, 2:5].double().cpu()
+    far = (dx[:, 2].double().cpu() - three.sum(1)).abs()
+    assert (far <= 4 * O.U * three.abs().sum(1) + torch.finfo(dtype).eps * three.sum(1).abs()).all()
+    # a NaN gate shows in its own channel from its step on, and nowhere else
+    bad = g.clone()
+    bad[0, 4, 3] = float("nan")
+    h, _ = gated_recurrence(x, bad, h0)
+    assert torch.isnan(h[0, 4:, 3]).all() and torch.isfinite(h[0, :4]).all() and torch.isfinite(h[0, :, :3]).all()
+
+
 def test_gated_recurrence_autograd_matches_explicit_gradients():
     from pearl_amd import gated_recurrence, gated_recurrence_grad
     c = recurrence_case(3, 100, 40, torch.float32, torch.float32, True, 41, lengths=True)
