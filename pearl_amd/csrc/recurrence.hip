@@ -22,7 +22,7 @@
 //
 // Where batch x channels give too few workgroups, the steps are cut into chunks: a first launch
 // composes each chunk's pair, the second starts every chunk from the composition of those before it
-// (1 x 65536 x 512 bf16: 32 + 42 us; the inputs are read twice).
+// (1 x 65536 x 512 bf16: 30 + 40 us; the inputs are read twice).
 //
 // Backward, with G_t = dh_t + c_t and c_{t-1} = a_t G_t (0 at a reset), c_T = d_last:
 //   decay:  dx = G, dg = G h_{t-1};   logit:  dx = (1 - a) G, dg = a (1 - a) G (h_{t-1} - x);
@@ -44,7 +44,7 @@ struct Shape {
 typedef Shape<1, 16, 8, 2> Short;          // histories of up to 32 steps
 typedef Shape<8, 16, 4, 2> Middle;         // of up to 128: half-width slabs (1 x 128 x 4096 fp32 6.2 us; as Long 14.4)
 typedef Shape<16, 32, 8, 2> Long;          // longer ones, forwards
-typedef Shape<8, 32, 8, 2> LongGrad;       // longer ones, backwards: 16 waves of 8 steps would spill (240 us, not 91)
+typedef Shape<8, 32, 8, 2> LongGrad;       // longer ones, backwards: 16 waves of 8 steps would spill (240 us, not 85)
 constexpr int KEEP = Long::STEPS / LongGrad::STEPS;
 static_assert(Short::SLAB <= 64 && Middle::SLAB <= 64 && Long::SLAB <= 64 && LongGrad::SLAB == Long::SLAB,
               "a lane of a wave carries the state of each channel");
@@ -436,7 +436,6 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       Tile<T, G, S> next;
       const Rows after = rows_of<S>(tile + 1 < tile1 ? tile + 1 : tile, n, a.reverse);
       load_rows<S, T, TINY>(next.x, xb, a.x_t, j, after, a.reverse, c);
-      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
       load_resets<S>(next.resets, a, b, j, after);
 
       // Most waves of most tiles have no reset and no step behind the end; without the selects for
@@ -474,6 +473,8 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       }
       if (lane >= 64 - CL) put_pair<V>(pairs, wave, slot, sA, sH, sR);
       __syncthreads();
+      // part of the next tile's loads only here: all at its start would leave the memory idle once they are in
+      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
       if (wave == 0) {
         join_waves<NW, SLAB, true, !EMIT>(pairs, lane, state, prod, forgot);
         if (EMIT && a.carries && owner) {
@@ -611,8 +612,6 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
       const int64_t tile_next = tile > tile0 ? tile - 1 : tile;
       const Rows after = rows_of<S>(tile_next, n, a.reverse);
       if constexpr (EMIT) load_rows<S, T, TINY>(next.x, xb, a.x_t, j, after, a.reverse, c);
-      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
-      load_rows<S, T, TINY>(dnext, db, d_t, j, after, a.reverse, c);
       load_resets<S>(next.resets, a, b, j, after);
       const float next_carry = EMIT && stater ? a.carries[(b * a.tiles + tile_next) * a.D + own] : 0.0f;
       if (!a.dh) {
@@ -696,9 +695,11 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
       if (lane < CL) put_pair<V>(bw, wave, slot, bA, C, bR);
       if (EMIT && lane >= 64 - CL) put_pair<V>(fw, wave, slot, A, H, fR);
       __syncthreads();
+      load_rows<S, G, TINY>(next.g, gb, a.g_t, j, after, a.reverse, c);
       if (wave == 0) join_waves<NW, SLAB, false, !EMIT>(bw, lane, back, prod, forgot);
       if (EMIT && wave == STATE_WAVE) join_waves<NW, SLAB, true, false>(fw, lane, carry, prod, forgot);
       __syncthreads();
+      load_rows<S, T, TINY>(dnext, db, d_t, j, after, a.reverse, c);
       if constexpr (EMIT) {
         const auto emit = [&](auto is_plain) {
           constexpr bool PLAIN = decltype(is_plain)::value;
