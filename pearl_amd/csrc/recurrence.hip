@@ -530,7 +530,8 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
   }
 }
 
-// One step, no scan: a lane per V channels.
+// One step, no scan: a lane per V channels, each channel one lane's alone, which reads its state before it
+// writes the new one: `last` may be h0.  (The kernels above read a row's last channels in two workgroups.)
 template <typename T, typename G, bool LOGIT>
 __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -555,7 +556,10 @@ __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
   }
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (a.last && v < left) a.last[b * a.D + c + v] = on ? h[v] : old[v];
+    if (v < left) {
+      if (a.carries) a.carries[b * a.D + c + v] = old[v];
+      if (a.last) a.last[b * a.D + c + v] = on ? h[v] : old[v];
+    }
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = on ? h[v] : 0.0f;
   const Pack<T, V> p = pack<T, V>(h);
@@ -803,7 +807,7 @@ Split split_of(int64_t B, int64_t T, int D, bool grad) {
 
 template <typename T, typename G, bool LOGIT, bool TINY>
 int run_forward(const RecArgs<T, G>& a, hipStream_t s) {
-  if (a.T_ == 1 && !a.carries) {
+  if (a.T_ == 1) {
     constexpr int V = 16 / (int)sizeof(T);
     hipLaunchKernelGGL((step_kernel<T, G, LOGIT>), dim3((unsigned)ceil_div(a.B * ceil_div(a.D, V), 256)),
                        dim3(256), 0, s, a);

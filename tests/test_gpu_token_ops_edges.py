@@ -1,0 +1,35 @@
+"""The token-policy operators on the GPU at the edges of what their interfaces allow.  Definitions and
+bounds: tests/token_oracle.py."""
+import pytest
+import torch
+
+import token_oracle as O
+from test_gpu_token_ops import DEV, DTYPES, IDS, gen_of, np64, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------- states written in place
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("b,d", [(1, 1), (3, 33), (200, 65), (5, 64), (70, 1025)])
+def test_single_step_that_keeps_states_and_writes_them_in_place(dtype, b, d):
+    """pa_gated_recurrence with T = 1, `last` = h0 and `carries`: every channel's old state is read, and kept
+    for the gradient, before the new one is written, also where a row's last channels share a pack."""
+    from pearl_amd import _native as N, gated_recurrence_grad
+    gen = gen_of(b, d, 91)
+    x, g, h0 = rnd(gen, b, 1, d, dtype=dtype), rnd(gen, b, 1, d, dtype=dtype), rnd(gen, b, d)
+    d_h, d_last = rnd(gen, b, 1, d, dtype=dtype), rnd(gen, b, d)
+    want = O.recurrence(np64(x), np64(g), np64(h0), None, None, True, False, np64(d_h), np64(d_last))
+    code = {torch.float32: N.PA_F32, torch.bfloat16: N.PA_BF16, torch.float16: N.PA_F16}[dtype]
+    assert N.lib().pa_gated_recurrence_carries(b, 1, d) == b * d
+    for _ in range(5):
+        state, kept, h = h0.clone(), torch.full((b * d,), float("nan"), device=DEV), torch.empty_like(x)
+        args = N.RECURRENCE_ARGS.pack(0, code, code, 1, 0, d, b, 1, x.data_ptr(), d, 0, g.data_ptr(), d, 0, state.data_ptr(),
+                                      0, 0, 0, 0, h.data_ptr(), state.data_ptr(), kept.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0)
+        N.check(N.lib().pa_gated_recurrence(args, N.stream_ptr(x.device)))
+        assert torch.equal(kept.view(b, d), h0)
+        O.check(h, *want["h"], dtype, "h")
+        O.check(state, *want["last"], torch.float32, "last")
+    dx, dg, d0 = gated_recurrence_grad(x, g, kept, d_h, d_last)
+    for got, name, kind in ((dx, "d_x", dtype), (dg, "d_g", dtype), (d0, "d_h0", torch.float32)):
+        O.check(got, *want[name], kind, name)
