@@ -1096,7 +1096,8 @@ typedef struct pa_recurrence_args {
   const int32_t* lengths;     /* [B], clamped to [0, T]; NULL: T.  Steps behind the end: h and
                                  gradients are 0, whatever x and gate hold there            */
   void* h;                    /* [B][T][D]                                                  */
-  float* last;                /* [B][D] state behind the last step; may be h0 when T = 1; NULL: not wanted */
+  float* last;                /* [B][D] state behind the last step; NULL: not wanted.  When T = 1 it may be
+                                 h0; any other overlap with an input is refused            */
   float* carries;             /* pa_gated_recurrence_carries floats: written by the forward pass for
                                  the gradient, read by it; NULL in a forward pass alone     */
   void* scratch;              /* pa_gated_recurrence_scratch bytes, 256-byte aligned        */

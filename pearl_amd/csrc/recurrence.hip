@@ -907,6 +907,26 @@ int check_args(const char* who, const pa_recurrence_args* p, bool grad) {
   return PA_OK;
 }
 
+// Whether `last` lies apart from what the pass reads.  A single step reads a channel before it writes it, so
+// there `last` may be h0, or x or the gate in the same layout; anything else would be read by some lanes after
+// others have written it.
+bool last_is_apart(const pa_recurrence_args* p) {
+  if (!p->last) return true;
+  const uintptr_t out = reinterpret_cast<uintptr_t>(p->last), out_end = out + p->B * p->D * 4;
+  const auto clear_of = [&](const void* in, int64_t last_element, int64_t size) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(in);
+    return !in || at >= out_end || at + (last_element + 1) * size <= out;
+  };
+  const auto rows_clear = [&](const void* in, int64_t b, int64_t t, int64_t size) {
+    const bool same = p->T == 1 && in == p->last && size == 4 && (b == p->D || p->B == 1);
+    return same || clear_of(in, (p->B - 1) * b + (p->T - 1) * t + p->D - 1, size);
+  };
+  return rows_clear(p->h0, p->D, 0, 4) && rows_clear(p->x, p->x_b, p->x_t, elem_size(p->dtype)) &&
+         rows_clear(p->gate, p->gate_b, p->gate_t, elem_size(p->gate_dtype)) &&
+         clear_of(p->resets, (p->B - 1) * p->resets_b + (p->T - 1) * p->resets_t, 1) &&
+         clear_of(p->lengths, p->B - 1, 4);
+}
+
 }  // namespace
 
 extern "C" int64_t pa_gated_recurrence_scratch(int64_t B, int64_t T, int32_t D) {
@@ -924,6 +944,7 @@ extern "C" int pa_gated_recurrence(const pa_recurrence_args* args, void* stream)
   if (rc != PA_OK) return rc;
   if (args->B == 0) return PA_OK;
   PA_REQUIRE(args->h, PA_ERR_INVALID, "pa_gated_recurrence: null output");
+  PA_REQUIRE(last_is_apart(args), PA_ERR_INVALID, "pa_gated_recurrence: the new state overlaps an input that is still read");
   PA_ON_DEVICE(args->device);
   return dispatch(args, false, reinterpret_cast<hipStream_t>(stream));
 }

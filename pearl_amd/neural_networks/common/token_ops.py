@@ -280,7 +280,7 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
                           out_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """One step of ``gated_recurrence`` for acting: x and gate (batch, channels), state float32 (batch,
     channels) or None for zeros, resets (batch).  Returns ``(h, new_state)``; ``out_state`` receives the new
-    state and may be ``state`` itself.  Records no backward pass and refuses inputs that ask for one."""
+    state and may be ``state`` itself; one that overlaps an input in another way is refused.  Records no backward pass and refuses inputs that ask for one."""
     op = "gated_recurrence_step"
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
             state is not None and state.requires_grad)):

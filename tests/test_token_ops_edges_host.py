@@ -1,0 +1,37 @@
+"""CPU: what the token-policy operators refuse at the edges of their interfaces.  No kernel runs here."""
+import ctypes as C
+
+
+
+def recurrence_args(N, **kw):
+    buf = C.cast((C.c_char * 65536)(), C.c_void_p).value
+    a = N.RecurrenceArgs()
+    a.dtype = a.gate_dtype = N.PA_BF16
+    a.B, a.T, a.D = 2, 1, 64
+    a.x_b = a.gate_b = 64
+    a.x, a.gate, a.h0, a.resets, a.lengths, a.h, a.last, a.scratch = (buf + 4096 * k for k in range(8))
+    a.resets_b = 1
+    a.device = 1000         # what passes the checks ends here
+    for k, v in kw.items():
+        setattr(a, k, a.last + v[0] if isinstance(v, tuple) else v)
+    return a
+
+
+def test_a_new_state_that_overlaps_what_is_read_is_refused():
+    from pearl_amd import _native as N
+    lib = N.lib()
+
+    def rc(**kw):
+        a = recurrence_args(N, **kw)
+        return lib.pa_gated_recurrence(C.byref(a), None)
+    passed = N.PA_ERR_HIP
+    assert rc() == rc(last=None) == rc(h0=None, resets=None, lengths=None) == passed
+    assert rc(h0=(0,)) == passed                                              # a single step in place
+    assert rc(h0=(512,)) == rc(h0=(-512,)) == passed                          # side by side
+    assert rc(x=(0,), dtype=N.PA_F32, gate_dtype=N.PA_F32) == passed          # read channel by channel as it is written
+    assert rc(x=(0,), dtype=N.PA_F32, gate_dtype=N.PA_F32, B=1, x_b=7) == passed
+    for bad in (dict(h0=(4,)), dict(h0=(-508,)), dict(h0=(0,), T=2), dict(x=(0,)), dict(x=(-128,)), dict(gate=(0,)),
+                dict(x=(0,), dtype=N.PA_F32, gate_dtype=N.PA_F32, x_b=65), dict(resets=(511,)), dict(lengths=(508,)),
+                dict(x=(0,), dtype=N.PA_F32, gate_dtype=N.PA_F32, T=2), dict(gate=(-510,), T=3, gate_t=64)):
+        assert rc(**bad) == N.PA_ERR_INVALID, bad
+        assert "overlaps" in N.last_error()
