@@ -1067,8 +1067,9 @@ int pa_embed_tokens(const void* weight, int32_t dtype, int64_t ldw, int64_t voca
                     const void* tokens, int32_t token_dtype, int64_t n, float scale, void* out,
                     int32_t device, void* stream);
 /* d_weight [vocab][dim] (written whole) = scale * sum over i with tokens[i] = v of d_out[i, :]: fp32
- * sums in index order, rounded once, the same bits for the same inputs.  Up to 2^26 tokens and rows.  scratch:
- * pa_embed_tokens_grad_scratch bytes, 256-byte aligned. */
+ * sums in index order, rounded once, the same bits for the same inputs.  Up to 2^26 tokens, 2^26
+ * rows and 2^46 of their product, which the time grows with (a third of a second there).
+ * scratch: pa_embed_tokens_grad_scratch bytes, 256-byte aligned. */
 int64_t pa_embed_tokens_grad_scratch(int64_t n, int32_t dim, int32_t dtype);
 int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ldd, const void* tokens,
                          int32_t token_dtype, int64_t n, float scale, int64_t vocab, int32_t dim,

@@ -82,7 +82,8 @@ def _embed(weight: Tensor, tokens: Tensor, scale: float) -> Tensor:
 
 
 def embed_tokens_grad(d_out: Tensor, tokens: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
-    """The gradient of ``embed_tokens`` with respect to its (vocab, dim) weight, in ``d_out``'s type."""
+    """The gradient of ``embed_tokens`` with respect to its (vocab, dim) weight, in ``d_out``'s type.  Up to 2^26
+    tokens, 2^26 rows and 2^46 tokens times rows: the time grows with that product (0.06 ms at 2^33, 5.5 at 2^40)."""
     code = dtype_code("embed_tokens_grad", "d_out", d_out, FLOATS)
     index = dtype_code("embed_tokens_grad", "tokens", tokens, INDICES)
     if d_out.dim() < 1 or d_out.shape[:-1] != tokens.shape:

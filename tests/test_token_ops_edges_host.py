@@ -35,3 +35,16 @@ def test_a_new_state_that_overlaps_what_is_read_is_refused():
                 dict(x=(0,), dtype=N.PA_F32, gate_dtype=N.PA_F32, T=2), dict(gate=(-510,), T=3, gate_t=64)):
         assert rc(**bad) == N.PA_ERR_INVALID, bad
         assert "overlaps" in N.last_error()
+
+
+def test_embedding_gradients_that_would_hold_the_card_are_refused():
+    from pearl_amd import _native as N
+    lib = N.lib()
+    buf = C.cast((C.c_char * 4096)(), C.c_void_p).value
+
+    def rc(n, vocab):
+        return lib.pa_embed_tokens_grad(buf, N.PA_F32, 4, buf, N.PA_I64, n, 1.0, vocab, 4, None, buf, 0, None)
+    for n, vocab in ((2 ** 26, 2 ** 20), (2 ** 20, 2 ** 26), (2 ** 23, 2 ** 23), (0, 2 ** 26), (1, 1)):
+        assert rc(n, vocab) == N.PA_ERR_INVALID          # no place for the result: past the limits
+    for n, vocab in ((2 ** 26, 2 ** 20 + 1), (2 ** 20 + 1, 2 ** 26), (2 ** 26, 2 ** 26)):
+        assert rc(n, vocab) == N.PA_ERR_UNSUPPORTED and "2^46" in N.last_error()
