@@ -9,7 +9,8 @@ libpearl_amd (embed.hip, recurrence.hip):
 Parameters and results are torch tensors in HBM (float32, bfloat16 or float16); work runs on the
 current stream of the tensors' device, which need not be the current device.  The functions record
 a backward pass when gradients are asked for; ``embed_tokens_grad`` and ``gated_recurrence_grad`` are
-the same kernels for learners that run their backward pass explicitly."""
+the same kernels for learners that run their backward pass explicitly.  None has a forward-mode derivative:
+inputs with a tangent are refused."""
 from __future__ import annotations
 
 from functools import lru_cache
@@ -17,6 +18,7 @@ from typing import Any, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ... import _native as N
@@ -33,6 +35,15 @@ def on_one_gpu(op: str, device: torch.device, *others: Optional[Tensor]) -> None
     for t in others:
         if t is not None and t.device != device:
             raise ValueError(f"{op}: tensors on {t.device} and on {device}")
+
+
+def no_tangents(op: str, *inputs: Optional[Tensor]) -> None:
+    """The kernels would drop the tangents of dual tensors without a word."""
+    if forward_ad._current_level < 0:       # no dual tensors anywhere: the usual case, at no cost
+        return
+    for t in inputs:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{op} has no forward-mode derivative")
 
 
 def dtype_code(op: str, name: str, t: Tensor, table: dict) -> int:
@@ -59,6 +70,7 @@ def embed_tokens(weight: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
     Token -1 stands for "none": a row of zeros that takes no part in the gradient.  Any other token
     outside the table gives a row of NaN; nothing is read for it.  The weight's gradient is dense,
     summed in float32 in the order of the tokens and the same bits for the same inputs."""
+    no_tangents("embed_tokens", weight)
     if weight.requires_grad and torch.is_grad_enabled():
         return _EmbedTokens.apply(weight, tokens, scale)
     return _embed(weight, tokens, scale)
@@ -84,6 +96,7 @@ def _embed(weight: Tensor, tokens: Tensor, scale: float) -> Tensor:
 def embed_tokens_grad(d_out: Tensor, tokens: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
     """The gradient of ``embed_tokens`` with respect to its (vocab, dim) weight, in ``d_out``'s type.  Up to 2^26
     tokens, 2^26 rows and 2^46 tokens times rows: the time grows with that product (0.06 ms at 2^33, 5.5 at 2^40)."""
+    no_tangents("embed_tokens_grad", d_out)
     code = dtype_code("embed_tokens_grad", "d_out", d_out, FLOATS)
     index = dtype_code("embed_tokens_grad", "tokens", tokens, INDICES)
     if d_out.dim() < 1 or d_out.shape[:-1] != tokens.shape:
@@ -137,6 +150,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor] = 
 
     Returns ``(h, last_state)``.  With ``keep=True`` no backward pass is recorded and a third result is
     what ``gated_recurrence_grad`` needs of the forward pass."""
+    no_tangents("gated_recurrence", x, gate, initial_state)
     if not keep and torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
             initial_state is not None and initial_state.requires_grad)):
         return _GatedRecurrence.apply(x, gate, initial_state, resets, lengths, gate_logits, reverse)
@@ -223,6 +237,7 @@ def gated_recurrence_grad(x: Tensor, gate: Tensor, kept: Tensor, d_h: Optional[T
     """Gradients ``(d_x, d_gate, d_initial_state)`` of ``gated_recurrence`` called with ``keep=True`` on the
     same x, gate, resets, lengths and flags, for the gradients of h and of the last state (None: zero)."""
     op = "gated_recurrence_grad"
+    no_tangents(op, x, gate, d_h, d_last)
     code, gate_code, xs, gs, resets, lengths = _inputs(op, x, gate, resets, lengths)
     b, t, d = x.shape
     if d_h is not None:
@@ -283,6 +298,7 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
     channels) or None for zeros, resets (batch).  Returns ``(h, new_state)``; ``out_state`` receives the new
     state and may be ``state`` itself; one that overlaps an input in another way is refused.  Records no backward pass and refuses inputs that ask for one."""
     op = "gated_recurrence_step"
+    no_tangents(op, x, gate, state)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
             state is not None and state.requires_grad)):
         raise RuntimeError(f"{op} records no backward pass: call it under torch.no_grad(), or gated_recurrence")

@@ -11,7 +11,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ... import _native as N
-from ..common.token_ops import FLOATS, INDICES, _address, dtype_code, on_one_gpu, scratch_of
+from ..common.token_ops import FLOATS, INDICES, _address, dtype_code, no_tangents, on_one_gpu, scratch_of
 
 
 class ActionLogProbs(NamedTuple):
@@ -31,7 +31,9 @@ def action_log_probs(logits: Tensor, actions: Tensor, unavailable_actions_mask: 
 
     A row without an available action has log_prob -inf, entropy 0, alternatives -1.  Action -1 stands for
     "none taken" (padding): log_prob 0.  Any other action outside [0, A) gives NaN.  log_prob and entropy are
-    differentiable with respect to the logits; the alternatives are not."""
+    differentiable with respect to the logits (backwards; logits with a forward-mode tangent are refused); the
+    alternatives are not."""
+    no_tangents("action_log_probs", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         out = _ActionLogProbs.apply(logits, actions, unavailable_actions_mask, temperature, top)
         return ActionLogProbs(*out)
@@ -104,6 +106,7 @@ def action_log_probs_grad(out: ActionLogProbs, logits: Tensor, actions: Tensor,
     """The logits' gradient, in their type, of ``action_log_probs`` called with the same arguments, for the
     float32 gradients of log_prob and of the entropy (None: zero)."""
     op = "action_log_probs_grad"
+    no_tangents(op, logits, d_log_prob, d_entropy)
     head, alive = _inputs(op, logits, actions, unavailable_actions_mask, temperature)
     device, shape, stats = logits.device, actions.shape, out.row_stats
     on_one_gpu(op, device, stats, d_log_prob, d_entropy)

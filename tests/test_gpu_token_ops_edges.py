@@ -2,6 +2,7 @@
 bounds: tests/token_oracle.py."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import token_oracle as O
 from test_gpu_token_ops import DEV, DTYPES, IDS, gen_of, np64, rnd
@@ -33,3 +34,20 @@ def test_single_step_that_keeps_states_and_writes_them_in_place(dtype, b, d):
     dx, dg, d0 = gated_recurrence_grad(x, g, kept, d_h, d_last)
     for got, name, kind in ((dx, "d_x", dtype), (dg, "d_g", dtype), (d0, "d_h0", torch.float32)):
         O.check(got, *want[name], kind, name)
+
+
+# ---------------------------------------------------------------------------- tangents
+def test_tangents_are_refused_and_plain_calls_beside_them_run():
+    from pearl_amd import action_log_probs, embed_tokens, gated_recurrence, gated_recurrence_step
+    x, tok = torch.randn(3, 4, 8, device=DEV), torch.tensor([[0, 1], [2, 2]], device=DEV)
+    w, act = torch.randn(3, 8, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    want = embed_tokens(w, tok)
+    with forward_ad.dual_level():
+        dual, wide = forward_ad.make_dual(w, torch.ones_like(w)), forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: embed_tokens(dual, tok), lambda: gated_recurrence(wide, x), lambda: gated_recurrence(x, wide),
+                     lambda: gated_recurrence(x, x, forward_ad.make_dual(x[:, 0], x[:, 1])),
+                     lambda: gated_recurrence_step(dual, w), lambda: action_log_probs(dual, act),
+                     lambda: gated_recurrence(wide.requires_grad_(), x)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(embed_tokens(w, tok), want)

@@ -1,6 +1,9 @@
 """CPU: what the token-policy operators refuse at the edges of their interfaces.  No kernel runs here."""
 import ctypes as C
 
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
 
 
 def recurrence_args(N, **kw):
@@ -48,3 +51,32 @@ def test_embedding_gradients_that_would_hold_the_card_are_refused():
         assert rc(n, vocab) == N.PA_ERR_INVALID          # no place for the result: past the limits
     for n, vocab in ((2 ** 26, 2 ** 20 + 1), (2 ** 20 + 1, 2 ** 26), (2 ** 26, 2 ** 26)):
         assert rc(n, vocab) == N.PA_ERR_UNSUPPORTED and "2^46" in N.last_error()
+
+
+def test_tangents_are_refused():
+    import pearl_amd as P
+    from pearl_amd._native import NativeError
+    w, tok = torch.randn(5, 4), torch.tensor([0, 1])
+    x, row = torch.randn(2, 6, 4), torch.randn(2, 4)
+    act, lp = torch.zeros(2, dtype=torch.int64), torch.zeros(2)
+    o = P.ActionLogProbs(lp, lp, None, None, torch.zeros(2, 3))
+    # every floating-point argument of every entry; plain tensors get as far as "no CPU fallback"
+    calls = [(lambda t: P.embed_tokens(t, tok), w), (lambda t: P.embed_tokens_grad(t, tok, 5), row),
+             (lambda t: P.gated_recurrence(t, x), x), (lambda t: P.gated_recurrence(x, t), x),
+             (lambda t: P.gated_recurrence(x, x, t), row), (lambda t: P.gated_recurrence(t, x, keep=True), x),
+             (lambda t: P.gated_recurrence_grad(t, x, w), x), (lambda t: P.gated_recurrence_grad(x, t, w), x),
+             (lambda t: P.gated_recurrence_grad(x, x, w, t), x), (lambda t: P.gated_recurrence_grad(x, x, w, x, t), row),
+             (lambda t: P.gated_recurrence_step(t, row), row), (lambda t: P.gated_recurrence_step(row, t), row),
+             (lambda t: P.gated_recurrence_step(row, row, t), row), (lambda t: P.action_log_probs(t, act), row),
+             (lambda t: P.action_log_probs_grad(o, t, act), row), (lambda t: P.action_log_probs_grad(o, row, act, t), lp),
+             (lambda t: P.action_log_probs_grad(o, row, act, lp, t), lp)]
+    for call, t in calls:
+        with pytest.raises(NativeError):
+            call(t)
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(NativeError):
+                call(t)
