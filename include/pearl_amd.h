@@ -1131,7 +1131,7 @@ typedef struct pa_log_probs_args {
   const void* actions;        /* [rows]                                                     */
   const uint8_t* mask;        /* 1 = unavailable; NULL: all are available                   */
   int64_t ldm;                /* bytes between rows; 0: one row for all                     */
-  float temperature;
+  float temperature;          /* 2^-126 .. 2^121                                            */
   int32_t top;                /* 0 .. 64 alternatives                                       */
   float* log_prob;            /* [rows]                                                     */
   float* entropy;             /* [rows]                                                     */

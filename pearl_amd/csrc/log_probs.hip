@@ -29,6 +29,9 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int MAX_TOP = 64;
+// Distances from the maximum are clamped at -FLT_MAX, which stands for -inf and for all that is further: up
+// to this temperature exp2(-FLT_MAX log2(e) / T) is zero (2^-184; at 1e38 it would be 0.03).
+constexpr float MAX_TEMPERATURE = 0x1p121f;
 
 template <typename T>
 struct LpArgs {
@@ -675,8 +678,8 @@ int check_args(const char* who, const pa_log_probs_args* p) {
              p->action_dtype);
   PA_REQUIRE(p->rows >= 0 && p->rows <= 0x7fffffffll && p->A >= 1 && p->ld >= 0 && p->ldm >= 0, PA_ERR_INVALID,
              "%s: bad shape (rows %lld, actions %d)", who, (long long)p->rows, p->A);
-  PA_REQUIRE(p->temperature >= FLT_MIN && p->temperature <= FLT_MAX, PA_ERR_INVALID, "%s: temperature %g", who,
-             (double)p->temperature);
+  PA_REQUIRE(p->temperature >= FLT_MIN && p->temperature <= MAX_TEMPERATURE, PA_ERR_INVALID,
+             "%s: temperature %g (2^-126 to 2^121)", who, (double)p->temperature);
   PA_REQUIRE(p->rows == 0 || (p->logits && p->actions), PA_ERR_INVALID, "%s: null pointer", who);
   return PA_OK;
 }

@@ -26,8 +26,8 @@ def action_log_probs(logits: Tensor, actions: Tensor, unavailable_actions_mask: 
                      temperature: float = 1.0, top: int = 0) -> ActionLogProbs:
     """For logits (..., A) and integer actions (...): log pi(action), the entropy of pi and, for ``top`` > 0,
     the ``top`` (at most 64) most probable actions with their log probabilities, in falling order with equal
-    logits by index.  pi = softmax(logits / temperature) over the available actions; the mask ((..., A) or
-    (A,), bool, True = unavailable) takes actions out, as does a logit of -inf.
+    logits by index.  pi = softmax(logits / temperature) over the available actions, for temperatures up to
+    2^121; the mask ((..., A) or (A,), bool, True = unavailable) takes actions out, as does a logit of -inf.
 
     A row without an available action has log_prob -inf, entropy 0, alternatives -1.  Action -1 stands for
     "none taken" (padding): log_prob 0.  Any other action outside [0, A) gives NaN.  log_prob and entropy are
@@ -51,8 +51,8 @@ def _inputs(op: str, logits: Tensor, actions: Tensor, mask: Optional[Tensor], te
     if not shape or shape[:-1] != actions.shape:
         raise ValueError(f"{op}: logits have shape {tuple(logits.shape)}, actions {tuple(actions.shape)}, "
                          "not (..., A) and (...)")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{op}: temperature {temperature}")
+    if not 0.0 < temperature <= 2.0 ** 121:
+        raise ValueError(f"{op}: temperature {temperature} (up to 2^121)")
     code, action_code = dtype_code(op, "logits", logits, FLOATS), dtype_code(op, "actions", actions, INDICES)
     width, rows = shape[-1], actions.numel()
     flat = logits if len(shape) == 2 else logits.reshape(rows, width)

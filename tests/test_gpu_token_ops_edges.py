@@ -5,7 +5,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import token_oracle as O
-from test_gpu_token_ops import DEV, DTYPES, IDS, gen_of, np64, rnd
+from test_gpu_token_ops import DEV, DTYPES, IDS, check_log_probs, gen_of, np64, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,21 @@ def test_tangents_are_refused_and_plain_calls_beside_them_run():
             with pytest.raises(NotImplementedError):
                 call()
         assert torch.equal(embed_tokens(w, tok), want)
+
+
+# ---------------------------------------------------------------------------- log probabilities
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("width", [10, 400, 9000])
+def test_action_log_probs_at_the_largest_and_smallest_temperature(dtype, width):
+    gen = gen_of(width, 81)
+    logits = rnd(gen, 6, width, dtype=dtype, scale=2.0)
+    mask = (torch.rand(6, width, generator=gen) < 0.4).to(DEV)
+    mask[:, 1] = False
+    logits[2, 2] = float("-inf")
+    logits[3, 3:] = torch.finfo(dtype).min
+    logits[4, 1] = torch.finfo(dtype).max
+    actions = torch.ones(6, dtype=torch.int64, device=DEV)
+    g_lp, g_h = rnd(gen, 6), rnd(gen, 6)
+    for temperature in (2.0 ** 121, 2.0 ** 60):
+        check_log_probs(logits, actions, mask, temperature, 4, dtype, g_lp, g_h, f"T {temperature}: ")
+        check_log_probs(logits, actions, None, temperature, 0, dtype, g_lp, None, f"T {temperature}, no mask: ")

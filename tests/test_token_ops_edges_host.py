@@ -80,3 +80,25 @@ def test_tangents_are_refused():
                 call(forward_ad.make_dual(t, torch.ones_like(t)))
             with pytest.raises(NativeError):
                 call(t)
+
+
+def test_temperatures_whose_distances_pass_a_float_are_refused():
+    """Above 2^121 the largest distance a float holds, divided by the temperature, no longer underflows in the
+    exponential: places that are not available would be counted."""
+    from pearl_amd import _native as N, action_log_probs
+    lib = N.lib()
+    buf = C.cast((C.c_char * 4096)(), C.c_void_p).value
+
+    def rc(entry, temperature):
+        a = N.LogProbsArgs()
+        a.dtype, a.action_dtype, a.A, a.rows, a.ld, a.temperature, a.device = N.PA_F32, N.PA_I64, 5, 2, 5, temperature, 1000
+        a.logits = a.actions = a.log_prob = a.entropy = a.stats = a.d_logits = buf
+        return entry(C.byref(a), None)
+    for entry in (lib.pa_action_log_probs, lib.pa_action_log_probs_grad):
+        assert rc(entry, 2.0 ** 121) == rc(entry, 2.0 ** -126) == N.PA_ERR_HIP      # past the checks
+        for far in (2.0 ** 121 * (1 + 2.0 ** -23), 1e37, 1e38, 3.4e38):
+            assert rc(entry, far) == N.PA_ERR_INVALID, far
+    for far in (2.0 ** 122, 1e38, 1e39, float("inf")):
+        with pytest.raises(ValueError):
+            action_log_probs(torch.randn(2, 5), torch.zeros(2, dtype=torch.int64), temperature=far)
+    assert 3.4028235e38 * 1.4427 / 2.0 ** 121 > 150 > 3.4028235e38 * 1.4427 / 1e38
