@@ -506,27 +506,43 @@ __device__ __forceinline__ RowGrad row_grad(const LpArgs<T>& a, int64_t row) {
   }
   return r;
 }
-// f: logits in (-inf: unavailable), gradients out.  With the row's constants gathered,
-//   dl = p (k0 + k1 log2 p),  k0 = -(g_lp + g_H H) / T,  k1 = -g_H ln 2 / T.
-// CHECK: the row is not an ordinary one (no action left, or NaN, which must not reach unavailable places).
+// What a row's elements share: dl = p (k0 + k1 log2 p), k0 = -(g_lp + g_H H), k1 = -g_H ln 2, over T.  In an
+// ordinary row everything is finite and k0, k1 hold the 1 / T already.
+constexpr float LOWEST = -1.0e4f;      // of log2 p: keeps p log p at zero where p has underflowed
+struct Factors {
+  float k0, k1, top;      // top: what the action taken gets on top
+};
+__device__ __forceinline__ Factors factors_of(const RowGrad& r, float inv_t) {
+  return {-fmaf(r.g_h, r.h, r.g_lp) * inv_t, -r.g_h * LN2 * inv_t, r.g_lp * inv_t};
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+__device__ __forceinline__ bool ordinary(const RowGrad& r, float inv_t) {
+  const Factors f = factors_of(r, inv_t);
+  return finite(r.m) && finite(r.h) && finite(f.k0) && finite(f.k1 * LOWEST) && finite(f.top);
+}
+// f: logits in (-inf: unavailable), gradients out.
+// CHECK: the row is not an ordinary one (no action left, NaN, or a factor that has no end): nothing of that
+// reaches unavailable places, and the division by T comes last, so that p = 0 gives 0 where only g / T passes
+// the range of a float.
 template <int N, bool CHECK>
 __device__ __forceinline__ void grad_of(float (&f)[N], int64_t j, const RowGrad& r, float c, float inv_t) {
-  const float k0 = -fmaf(r.g_h, r.h, r.g_lp) * inv_t, k1 = -r.g_h * LN2 * inv_t;
+  const float by = CHECK ? 1.0f : inv_t;
+  const Factors k = factors_of(r, by);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    // the clamp keeps p log p at zero where p has underflowed
-    const float t2 = fmaxf(fmaf(f[i] - r.m, c, -r.log2s), -1.0e4f);
-    const float d = __builtin_amdgcn_exp2f(t2) * fmaf(k1, t2, k0);
+    const float t2 = fmaxf(fmaf(f[i] - r.m, c, -r.log2s), LOWEST), p = __builtin_amdgcn_exp2f(t2);
+    const float d = p * fmaf(k.k1, CHECK && p == 0.0f ? 1.0f : t2, k.k0);
     f[i] = CHECK && (f[i] == -INFINITY || r.none) ? 0.0f : d;
   }
   if (r.t >= j && r.t < j + N) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (j + i == r.t) f[i] = fmaf(r.g_lp, inv_t, f[i]);
+      if (j + i == r.t) f[i] = fmaf(r.g_lp, by, f[i]);
   }
-}
-__device__ __forceinline__ bool ordinary(const RowGrad& r) {
-  return r.m > -INFINITY && r.m < INFINITY && r.h == r.h && r.g_lp == r.g_lp && r.g_h == r.g_h;
+  if constexpr (CHECK) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] *= inv_t;
+  }
 }
 
 template <typename T>
@@ -575,7 +591,7 @@ __global__ __launch_bounds__(256) void large_grad_kernel(LpArgs<T> a) {
         if (j < a.A) store_pack<T, V>(dst + at, pack<T, V>(f));
       }
     };
-    if (ordinary(r)) write(Bool<false>());
+    if (ordinary(r, a.inv_t)) write(Bool<false>());
     else write(Bool<true>());
   }
 }

@@ -69,3 +69,57 @@ def test_action_log_probs_at_the_largest_and_smallest_temperature(dtype, width):
     for temperature in (2.0 ** 121, 2.0 ** 60):
         check_log_probs(logits, actions, mask, temperature, 4, dtype, g_lp, g_h, f"T {temperature}: ")
         check_log_probs(logits, actions, None, temperature, 0, dtype, g_lp, None, f"T {temperature}, no mask: ")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("width", [10, 400, 9000])
+def test_action_log_probs_infinite_gradients_stay_away_from_unavailable_actions(dtype, width):
+    from pearl_amd import action_log_probs, action_log_probs_grad
+    inf = float("inf")
+    gen = gen_of(width, 83)
+    logits = rnd(gen, 6, width, dtype=dtype, scale=2.0)
+    mask = (torch.rand(6, width, generator=gen) < 0.4).to(DEV)
+    mask[:, 2] = False
+    logits[:, 7] = float("-inf")
+    off = mask | (logits == float("-inf"))
+    actions = torch.full((6,), 2, device=DEV)
+    g_lp, g_h = rnd(gen, 6), rnd(gen, 6)
+    o = action_log_probs(logits, actions, mask)
+    plain = action_log_probs_grad(o, logits, actions, g_lp, g_h, mask)
+    g_lp[0], g_h[1], g_lp[2], g_h[3] = inf, inf, -inf, float("nan")
+    for some in ((g_lp, g_h), (g_lp, None), (None, g_h)):
+        d = action_log_probs_grad(o, logits, actions, *some, mask)
+        assert (d[off] == 0).all()
+        assert torch.isfinite(d[4:]).all()
+    d = action_log_probs_grad(o, logits, actions, g_lp, g_h, mask)
+    assert torch.equal(d[4:], plain[4:])
+    on = ~off
+    on[:, 2] = False
+    assert (d[0][on[0]] == -inf).all() and (d[2][on[2]] == inf).all() and torch.isnan(d[3][on[3]]).all()
+
+
+@pytest.mark.parametrize("width", [10, 400, 9000])
+def test_action_log_probs_gradients_that_overflow_leave_the_others_alone(width):
+    """g / T passes the range of a float: where p or 1 - p is zero the gradient is zero all the same."""
+    from pearl_amd import action_log_probs, action_log_probs_grad
+    logits = -torch.arange(width, device=DEV, dtype=torch.float32).repeat(2, 1) - 1.0
+    actions = torch.tensor([0, 1], device=DEV)
+    o = action_log_probs(logits, actions, temperature=2.0e-38)      # distances of 5e37 and more: p is 1, 0, 0, ...
+    d = action_log_probs_grad(o, logits, actions, torch.full((2,), 10.0, device=DEV), temperature=2.0e-38)
+    want = torch.zeros(2, width, device=DEV)
+    want[1, 0], want[1, 1] = float("-inf"), float("inf")
+    assert torch.equal(d, want)
+
+
+def test_action_log_probs_the_largest_entropy_gradients():
+    """g_H (log p + H) passes the range of a float for every p that has underflowed, and only there counts for nothing."""
+    from pearl_amd import action_log_probs, action_log_probs_grad
+    for width in (10, 400, 9000):
+        logits = torch.full((2, width), -1000.0, device=DEV)
+        logits[:, 0] = 0.0
+        logits[:, 1] = float("-inf")
+        actions = torch.zeros(2, dtype=torch.int64, device=DEV)
+        o = action_log_probs(logits, actions)
+        for g in (3.0e38, 1.0e35):
+            d = action_log_probs_grad(o, logits, actions, None, torch.full((2,), g, device=DEV))
+            assert (d == 0).all(), (width, g)
