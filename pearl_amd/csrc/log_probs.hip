@@ -150,6 +150,12 @@ __device__ __forceinline__ float logit_of(const LpArgs<T>& a, int64_t row, int64
   return (float)a.logits[row * a.ld + j];
 }
 
+// log p of a logit below (or at) the maximum.  The distance is taken in halves: between the ends of the range it
+// would pass it, where divided by T it need not.
+__device__ __forceinline__ float log_prob_of(float v, float m, float inv_t, float log_s) {
+  return (0.5f * v - 0.5f * m) * inv_t * 2.0f - log_s;
+}
+
 // one lane per row writes what the sums say
 template <typename T>
 __device__ __forceinline__ void finish_row(const LpArgs<T>& a, int64_t row, const Sums& x, float& log_s) {
@@ -163,7 +169,7 @@ __device__ __forceinline__ void finish_row(const LpArgs<T>& a, int64_t row, cons
   else if (t < 0 || t >= a.A) lp = __builtin_nanf("");
   else {
     const float v = logit_of(a, row, t);
-    lp = bad ? __builtin_nanf("") : v == -INFINITY ? -INFINITY : (v - x.m) * a.inv_t - log_s;
+    lp = bad ? __builtin_nanf("") : v == -INFINITY ? -INFINITY : log_prob_of(v, x.m, a.inv_t, log_s);
   }
   a.log_prob[row] = lp;
   a.entropy[row] = h;
@@ -177,7 +183,7 @@ template <typename T>
 __device__ __forceinline__ void write_top(const LpArgs<T>& a, int64_t row, int k, uint64_t key, const Sums& x,
                                           float log_s) {
   a.top_actions[row * a.top + k] = key ? (int64_t)(uint32_t)~(uint32_t)key : -1;
-  a.top_log_probs[row * a.top + k] = key ? (value_of(key) - x.m) * a.inv_t - log_s : -INFINITY;
+  a.top_log_probs[row * a.top + k] = key ? log_prob_of(value_of(key), x.m, a.inv_t, log_s) : -INFINITY;
 }
 
 // ---- up to 256 actions: a few lanes per row, four actions per lane, all in registers ---------------

@@ -123,3 +123,15 @@ def test_action_log_probs_the_largest_entropy_gradients():
         for g in (3.0e38, 1.0e35):
             d = action_log_probs_grad(o, logits, actions, None, torch.full((2,), g, device=DEV))
             assert (d == 0).all(), (width, g)
+
+
+@pytest.mark.parametrize("width", [10, 400, 20000])
+def test_action_log_probs_of_logits_further_apart_than_a_float_holds(width):
+    gen = gen_of(width, 82)
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = rnd(gen, 4, width, dtype=dtype)
+        logits[:, 0] = 3.2e38
+        logits[1, 1:] = -3.2e38
+        logits[2, 5] = -3.0e38
+        actions = torch.tensor([0, 3, 5, 5], device=DEV)
+        check_log_probs(logits, actions, None, 16.0, 4, dtype, rnd(gen, 4), rnd(gen, 4), "far: ")
