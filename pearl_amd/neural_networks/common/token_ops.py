@@ -20,6 +20,7 @@ import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from ... import _native as N
 
@@ -300,7 +301,7 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
     op = "gated_recurrence_step"
     no_tangents(op, x, gate, state)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (
-            state is not None and state.requires_grad)):
+            state is not None and state.requires_grad) or (out_state is not None and out_state.requires_grad)):
         raise RuntimeError(f"{op} records no backward pass: call it under torch.no_grad(), or gated_recurrence")
     shape = x.shape
     if len(shape) != 2 or gate.shape != shape:
@@ -326,6 +327,8 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
     h = torch.empty(b, d, dtype=x.dtype, device=device)
     if out_state is None:
         out_state = torch.empty(b, d, dtype=torch.float32, device=device)
+    elif not out_state.is_inference():      # such tensors have no versions
+        increment_version(out_state)        # or a backward pass that kept the old state would read the new one
     if b * d:
         args = N.RECURRENCE_ARGS.pack(
             device.index, code, gate_code, bool(gate_logits), False, d, b, 1,

@@ -135,3 +135,20 @@ def test_action_log_probs_of_logits_further_apart_than_a_float_holds(width):
         logits[2, 5] = -3.0e38
         actions = torch.tensor([0, 3, 5, 5], device=DEV)
         check_log_probs(logits, actions, None, 16.0, 4, dtype, rnd(gen, 4), rnd(gen, 4), "far: ")
+
+
+def test_a_state_written_in_place_is_known_to_autograd():
+    from pearl_amd import gated_recurrence_step
+    x, g, state = (torch.randn(3, 8, device=DEV) for _ in range(3))
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    y = (state * w).sum()                                     # keeps the state for w's gradient
+    gated_recurrence_step(x, g, state, out_state=state)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        kept = torch.zeros(3, 8, device=DEV)
+    for _ in range(2):
+        gated_recurrence_step(x, g, kept, out_state=kept)      # made in inference mode: nothing to tell
+    leaf = torch.zeros(3, 8, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError):
+        gated_recurrence_step(x, g, out_state=leaf)
