@@ -61,7 +61,7 @@ struct RecArgs {
   int reverse;
   int slabs, chunks; int64_t chunk_tiles, tiles;
   int64_t kept;                                  // states kept per history: the gradient's tiles
-  float* agg_a; float* agg_h; uint8_t* agg_r;    // [B][chunks][D], [B][chunks]: the chunks' pairs
+  float* agg_a; float* agg_h; uint8_t* agg_r;    // [B][chunks][D], [B][chunks][slabs]: the chunks' pairs
   T* h; float* last; float* carries;             // [B][T][D], [B][D] or null, [B][tiles][D] or null
   const T* dh; int64_t dh_b, dh_t;               // or null: zeros
   const float* d_last;                           // [B][D] or null
@@ -232,6 +232,18 @@ __device__ __forceinline__ int channel_of(int first, int D) {
   return TINY ? first : first < D - V ? first : D - V;
 }
 
+// The channels of a workgroup: SLAB of them.  With decays, where the last slab would hold a single one, it takes
+// two more from the one before, so that a pack moved back shares its channels with a lane of its own workgroup
+// only: one of two workgroups may walk its tiles twice, which rounds differently.
+struct Slab {
+  int first, width;
+};
+template <typename S, bool LOGIT>
+__device__ __forceinline__ Slab slab_of(int slab, int slabs, int D) {
+  const int taken = !LOGIT && slabs > 1 && D % S::SLAB == 1 ? S::V : 0;
+  return {slab * S::SLAB - (slab == slabs - 1 ? taken : 0), S::SLAB - (slab == slabs - 2 ? taken : 0)};
+}
+
 // the factor and the input of one step; PLAIN: the step is known to lie inside the history
 template <typename T, typename G, int V, bool LOGIT, bool PLAIN>
 __device__ __forceinline__ void step_of(const Pack<T, V>& px, const Pack<G, V>& pg, bool on, float (&a)[V],
@@ -345,18 +357,144 @@ __device__ __forceinline__ void join_waves(Pairs<NW, SLAB>& p, int lane, float& 
   }
 }
 
+// ---- decays above one --------------------------------------------------------------------------------
+// A product of many decays above one passes the range of a float though the states stay inside it: a state of
+// zero, or a small one, or decays that shrink again, and infinity times zero is no state.  Where a workgroup
+// has met a decay above 1 in size it walks its tiles a second time, with products kept as A 2^E, A between 1/2
+// and 1: every group of lanes takes its steps one after another, and one wave takes the groups.  A walk of its
+// own, behind the other and in rolled loops: the same arithmetic within the one loop cost histories without such
+// decays 8 to 14 % (registers: their loop uses all it may), the look at the decays costs 0 to 2 % (16 x 2048 x 1024
+// fp32 forwards 84.9 -> 86.8 us, bf16 35.7 both) and 1 us where a short history is cut.
+__device__ __forceinline__ void normalise(float& A, int& E) {
+  const int e = E + __builtin_amdgcn_frexp_expf(A);      // zero, infinity and NaN: 0
+  A = __builtin_amdgcn_frexp_mantf(A);
+  E = e < -(1 << 24) ? -(1 << 24) : e > (1 << 24) ? 1 << 24 : e;
+}
+__device__ __forceinline__ float apply_wide(float A, int E, float s, float H) {
+  return __builtin_ldexpf(A * s, E) + H;
+}
+
+// Whether a lane holds a decay above 1 in size.  Of 16-bit ones by their bits, two at once: added to what one lacks
+// to the next power of two, everything above one reaches that exponent's top bit, one itself does not.  (A NaN
+// may pass unseen; it is a NaN in either walk.)
+template <typename G, int V, int L>
+__device__ __forceinline__ bool grows(const Pack<G, V> (&g)[L]) {
+  if constexpr (sizeof(G) == 4) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) most = fmaxf(most, fabsf(__uint_as_float(g[i].w[v])));
+    return most > 1.0f;
+  } else {
+    constexpr uint32_t lacks = __is_same(G, bf16_t) ? 0x4000 - 0x3f80 - 1 : 0x4000 - 0x3c00 - 1;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+#pragma unroll
+      for (int k = 0; k < Pack<G, V>::WORDS; ++k) top |= g[i].w[k] + (lacks << 16 | lacks);
+    return (top & 0x40004000u) != 0;
+  }
+}
+
+// The pairs of all groups of a tile and the states in front of them.
+template <int GROUPS, int SLAB>
+struct WidePairs {
+  float A[GROUPS][SLAB], H[GROUPS][SLAB], in[GROUPS][SLAB];
+  int E[GROUPS][SLAB], R[GROUPS];
+};
+template <int V, int GROUPS, int SLAB>
+__device__ __forceinline__ void put_wide(WidePairs<GROUPS, SLAB>& p, int group, int slot, const float (&A)[V], const int (&E)[V],
+                                         const float (&H)[V], bool R) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    p.A[group][slot + v] = A[v];
+    p.H[group][slot + v] = H[v];
+    p.E[group][slot + v] = E[v];
+  }
+  p.R[group] = R;
+}
+template <int GROUPS, int SLAB, bool UP, bool PROD>
+__device__ __forceinline__ void walk_wide(WidePairs<GROUPS, SLAB>& p, int lane, float& state, float& prod, int& prod_e,
+                                          bool& forgot) {
+  if (lane >= SLAB) return;
+#pragma unroll 1
+  for (int k = 0; k < GROUPS; ++k) {
+    const int w = UP ? k : GROUPS - 1 - k;
+    const float A = p.A[w][lane], H = p.H[w][lane];
+    const int E = p.E[w][lane];
+    const bool r = p.R[w];
+    p.in[w][lane] = state;
+    state = r ? H : apply_wide(A, E, state, H);
+    if constexpr (PROD) {
+      prod = r ? 0.0f : prod * A;
+      prod_e = r ? 0 : prod_e + E;
+      normalise(prod, prod_e);
+      forgot = forgot || r;
+    }
+  }
+}
+// behind agg_h, as far as that is behind agg_a
+template <typename T, typename G>
+__device__ __forceinline__ int32_t* exponents(const RecArgs<T, G>& a) {
+  return reinterpret_cast<int32_t*>(a.agg_h + (a.agg_h - a.agg_a));
+}
+// A chunk's pair is kept with its exponent; bit 0 of its byte: a reset, bit 1: some exponent is not 0.
+enum { CHUNK_RESET = 1, CHUNK_WIDE = 2 };
+template <typename T, typename G, bool LOGIT>
+__device__ __forceinline__ void put_chunk(const RecArgs<T, G>& a, int64_t b, int slab, int chunk, int lane, int own, float A,
+                                          int E, float H, bool reset) {
+  const int64_t o = b * a.chunks + chunk;
+  a.agg_a[o * a.D + own] = A;
+  a.agg_h[o * a.D + own] = H;
+  if constexpr (!LOGIT) exponents(a)[o * a.D + own] = E;
+  const bool wide = !LOGIT && __any(E != 0);
+  if (lane == 0) a.agg_r[o * a.slabs + slab] = (reset ? CHUNK_RESET : 0) | (wide ? CHUNK_WIDE : 0);
+}
+// A channel's state taken through the chunks in front of this one (UP; behind it, down), one after another.
+template <typename T, typename G, bool UP>
+__device__ __forceinline__ void walk_chunks(const RecArgs<T, G>& a, int64_t b, int slab, int chunk, int own, float& state) {
+  const int first = UP ? 0 : chunk + 1, last = UP ? chunk : a.chunks;
+#pragma unroll 1
+  for (int k = 0; k < last - first; ++k) {
+    const int64_t o = b * a.chunks + (UP ? first + k : last - 1 - k), at = o * a.D + own;
+    const float H = a.agg_h[at];
+    state = a.agg_r[o * a.slabs + slab] & CHUNK_RESET ? H : apply_wide(a.agg_a[at], exponents(a)[at], state, H);
+  }
+}
+// A lane's place in the slab, as the kernels below compute it, but from an index that the compiler takes for
+// another: its values need not live through their loops.
+template <typename S, bool TINY>
+struct Place {
+  int lane, wave, slot, c, own, group;
+  bool active, owner;
+  __device__ __forceinline__ Place(int slab, int slabs, int D) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    lane = tid & 63;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    slot = (lane & (S::CL - 1)) * S::V;
+    const Slab mine = slab_of<S, false>(slab, slabs, D);
+    active = slot < mine.width && mine.first + slot < D;
+    c = active ? channel_of<S::V, TINY>(mine.first + slot, D) : 0;
+    own = channel_of<S::V, TINY>(mine.first + lane / S::V * S::V, D) + lane % S::V;
+    owner = wave == 0 && lane < mine.width && mine.first + lane / S::V * S::V < D && own < D;
+    group = wave * S::TG + lane / S::CL;
+  }
+};
+
 // The state in front of a chunk: the composition of the chunks before it (UP; behind it, down), scanned
 // like steps, one chunk per group of lanes.
-template <typename T, typename G, typename S, bool UP, bool TINY>
-__device__ __forceinline__ void through_chunks(const RecArgs<T, G>& a, Pairs<S::NW, S::SLAB>& pairs, int64_t b, int chunk,
-                                               int lane, int wave, int slot, int c, float& state) {
+template <typename T, typename G, typename S, bool DECAY, bool UP, bool TINY>
+__device__ __forceinline__ void through_chunks(const RecArgs<T, G>& a, Pairs<S::NW, S::SLAB>& pairs, int64_t b, int slab,
+                                               int chunk, int lane, int wave, int slot, int c, bool& grown, float& state) {
   constexpr int V = S::V, GROUPS = S::NW * S::TG;
   const int first = UP ? 0 : chunk + 1, last = UP ? chunk : a.chunks;     // [first, last)
   for (int done = 0; done < last - first; done += GROUPS) {
     const int g = wave * S::TG + lane / S::CL;
     const int k = UP ? first + done + g : last - 1 - done - (GROUPS - 1 - g);
     float A[V], H[V], prod = 0.0f;
-    bool R = false, forgot = false;
+    bool R = false, forgot = false, wide = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       A[v] = 1.0f;
@@ -370,8 +508,11 @@ __device__ __forceinline__ void through_chunks(const RecArgs<T, G>& a, Pairs<S::
           A[v] = a.agg_a[o * a.D + c + v];
           H[v] = a.agg_h[o * a.D + c + v];
         }
-      R = a.agg_r[o];
+      const int flags = a.agg_r[o * a.slabs + slab];
+      R = flags & CHUNK_RESET;
+      if (DECAY && (flags & CHUNK_WIDE)) wide = true;
     }
+    if (DECAY) grown = grown || __any(wide);
     wave_scan<V, S::CL, UP, false>(A, H, R, lane);
     if (UP ? lane >= 64 - S::CL : lane < S::CL) put_pair<V>(pairs, wave, slot, A, H, R);
     __syncthreads();
@@ -400,19 +541,123 @@ struct Bool {
   static constexpr bool value = B;
 };
 
+// Step k of a tile's rows, loaded by itself: in the rolled loops below few registers are held, as the loops that
+// have no decays above one would otherwise spill theirs.
+template <typename S, typename T, bool TINY>
+__device__ __forceinline__ Pack<T, S::V> load_step(const T* base, int64_t stride, int k, const Rows& r, int reverse, int c) {
+  return buffer_load<T, S::V, TINY>(buffer_at(base + r.first * stride),
+                                    row_offset(k, r, reverse, (uint32_t)(stride * sizeof(T)), (uint32_t)(c * sizeof(T))), 0);
+}
+template <typename T, typename G>
+__device__ __forceinline__ bool reset_at(const RecArgs<T, G>& a, int64_t b, int k, const Rows& r) {
+  return a.resets && k < r.valid && a.resets[b * a.r_b + (r.first + (a.reverse ? r.here - 1 - k : k)) * a.r_t];
+}
+// one lane's pair
+template <int V>
+struct WidePair {
+  float A[V], H[V];
+  int E[V];
+  bool R;
+  __device__ __forceinline__ WidePair() : R(false) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      A[v] = 1.0f;
+      H[v] = 0.0f;
+      E[v] = 0;
+    }
+  }
+  __device__ __forceinline__ void add(const float (&f)[V], const float (&in)[V], bool r) {
+    R = R || r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      H[v] = r ? in[v] : fmaf(f[v], H[v], in[v]);
+      A[v] = r ? 0.0f : A[v] * f[v];
+      normalise(A[v], E[v]);
+    }
+  }
+};
+
+// The tiles of a chunk of a history among whose decays some are above one.
+template <typename T, typename G, typename S, bool EMIT, bool TINY>
+__device__ __forceinline__ void wide_tiles(const RecArgs<T, G>& a, WidePairs<S::NW * S::TG, S::SLAB>& pairs, int64_t b, int64_t n,
+                                           int slab, int chunk, int64_t tile0, int64_t tile1, float& state, float& prod,
+                                           int& prod_e, bool& forgot) {
+  constexpr int V = S::V, L = S::L, GROUPS = S::NW * S::TG;
+  const Place<S, TINY> me(slab, a.slabs, a.D);
+  const int lane = me.lane, wave = me.wave, slot = me.slot, c = me.c, own = me.own, group = me.group, j = group * L;
+  state = EMIT && me.owner && a.h0 ? a.h0[b * a.D + own] : 0.0f;
+  prod = 1.0f;
+  prod_e = 0;
+  forgot = false;
+  if (EMIT && me.owner) walk_chunks<T, G, true>(a, b, slab, chunk, own, state);
+#pragma unroll 1
+  for (int64_t tile = tile0; tile < tile1; ++tile) {
+    const Rows rows = rows_of<S>(tile, n, a.reverse);
+    float f[V], keep[V], x[V], in[V];
+    const auto step = [&](int k) {
+      const Pack<T, V> px = load_step<S, T, TINY>(a.x + b * a.x_b, a.x_t, k, rows, a.reverse, c);
+      const Pack<G, V> pg = load_step<S, G, TINY>(a.g + b * a.g_b, a.g_t, k, rows, a.reverse, c);
+      step_of<T, G, V, false, false>(px, pg, k < rows.valid, f, keep, x, in);
+      return reset_at(a, b, k, rows);
+    };
+    WidePair<V> p;
+#pragma unroll 1
+    for (int k = j; k < j + L; ++k) {
+      const bool r = step(k);
+      p.add(f, in, r);
+    }
+    __syncthreads();        // the pairs of the tile before are done with
+    put_wide<V>(pairs, group, slot, p.A, p.E, p.H, p.R);
+    __syncthreads();
+    if (wave == 0) {
+      walk_wide<GROUPS, S::SLAB, true, !EMIT>(pairs, lane, state, prod, prod_e, forgot);
+      if (EMIT && a.carries && me.owner) {
+        constexpr int PARTS = S::STEPS == Long::STEPS ? KEEP : 1;
+#pragma unroll 1
+        for (int q = 0; q < PARTS; ++q)
+          if (tile * PARTS + q < a.kept)
+            a.carries[(b * a.kept + tile * PARTS + q) * a.D + own] = pairs.in[q * (GROUPS / PARTS)][lane];
+      }
+    }
+    if constexpr (EMIT) {
+      __syncthreads();
+      if (me.active) {
+        float s[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = pairs.in[group][slot + v];
+#pragma unroll 1
+        for (int k = j; k < j + L; ++k) {
+          const bool r = step(k);
+          float h[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            s[v] = r ? in[v] : fmaf(f[v], s[v], in[v]);
+            h[v] = k < rows.valid ? s[v] : 0.0f;
+          }
+          const int64_t at = tile * S::STEPS + k;
+          if (at < a.T_) put_step<S, T, TINY>(a.h + b * a.T_ * a.D, at, n, a.reverse, c, a.D, pack<T, V>(h));
+        }
+      }
+    }
+  }
+}
+
 // LOGIT gates or decay gates; EMIT: states out, else the pair of a chunk alone
 template <typename T, typename G, typename S, bool LOGIT, bool EMIT, bool TINY>
 __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a) {
   constexpr int V = S::V, SLAB = S::SLAB, NW = S::NW, CL = S::CL, L = S::L;
   __shared__ Pairs<NW, SLAB> pairs;
+  __shared__ WidePairs<LOGIT ? 1 : NW * S::TG, SLAB> wide;
+  __shared__ int wave_grown[NW];      // decays: one above 1 in a wave's steps so far, or a wide chunk in front of them
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs, chunk = blockIdx.x / a.slabs;
   const int slot = (lane & (CL - 1)) * V;
-  const bool active = slab * SLAB + slot < a.D;
-  const int c = active ? channel_of<V, TINY>(slab * SLAB + slot, a.D) : 0;
+  const Slab mine = slab_of<S, LOGIT>(slab, a.slabs, a.D);
+  const bool active = slot < mine.width && mine.first + slot < a.D;
+  const int c = active ? channel_of<V, TINY>(mine.first + slot, a.D) : 0;
   // lane k of wave 0 carries the state of this channel
-  const int own = channel_of<V, TINY>(slab * SLAB + lane / V * V, a.D) + lane % V;
-  const bool owner = wave == 0 && lane < SLAB && slab * SLAB + lane / V * V < a.D && own < a.D;
+  const int own = channel_of<V, TINY>(mine.first + lane / V * V, a.D) + lane % V;
+  const bool owner = wave == 0 && lane < mine.width && mine.first + lane / V * V < a.D && own < a.D;
   const int j = (wave * S::TG + lane / CL) * L;             // this lane's first step in a tile
   const int64_t tile0 = chunk * a.chunk_tiles;
   const int64_t tile1 = tile0 + a.chunk_tiles < a.tiles ? tile0 + a.chunk_tiles : a.tiles;
@@ -430,8 +675,9 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
     load_rows<S, G, TINY>(cur.g, gb, a.g_t, j, rows, a.reverse, c);
     load_resets<S>(cur.resets, a, b, j, rows);
     float state = EMIT && owner && a.h0 ? a.h0[b * a.D + own] : 0.0f, prod = 1.0f;
-    bool forgot = false;
-    if (EMIT && chunk) through_chunks<T, G, S, true, TINY>(a, pairs, b, chunk, lane, wave, slot, c, state);
+    bool forgot = false, grown = false;
+    if (EMIT && chunk) through_chunks<T, G, S, !LOGIT, true, TINY>(a, pairs, b, slab, chunk, lane, wave, slot, c, grown, state);
+    if constexpr (!LOGIT) wave_grown[wave] = grown;
     for (int64_t tile = tile0; tile < tile1; ++tile) {
       Tile<T, G, S> next;
       const Rows after = rows_of<S>(tile + 1 < tile1 ? tile + 1 : tile, n, a.reverse);
@@ -440,7 +686,10 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
 
       // Most waves of most tiles have no reset and no step behind the end; without the selects for
       // those a step costs half the instructions.
-      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets));
+      bool above = false;
+      if constexpr (!LOGIT) above = grows<G, V, L>(cur.g);
+      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets) || above);
+      if (!LOGIT && !plain && __any(above)) wave_grown[wave] = 1;
       uint32_t resets = 0;
       float A[L][V], H[L][V], sA[V], sH[V];
       bool sR = false;
@@ -517,21 +766,24 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       cur = next;
       rows = after;
     }
+    int prod_e = 0;
+    if constexpr (!LOGIT) {
+      if (__any(lane < NW && wave_grown[lane & (NW - 1)]))       // the same answer in every wave
+        wide_tiles<T, G, S, EMIT, TINY>(a, wide, b, n, slab, chunk, tile0, tile1, state, prod, prod_e, forgot);
+      if (b + gridDim.y < a.B) __syncthreads();                  // before the flags are written again
+    }
     if (owner) {
       if constexpr (EMIT) {
         if (a.last && chunk == a.chunks - 1) a.last[b * a.D + own] = state;
       } else {
-        const int64_t o = b * a.chunks + chunk;
-        a.agg_a[o * a.D + own] = prod;
-        a.agg_h[o * a.D + own] = state;
-        if (lane == 0) a.agg_r[o] = forgot;     // the same in every slab
+        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, state, forgot);
       }
     }
   }
 }
 
 // One step, no scan: a lane per V channels, each channel one lane's alone, which reads its state before it
-// writes the new one: `last` may be h0.  (The kernels above read a row's last channels in two workgroups.)
+// writes the new one: `last` may be h0.
 template <typename T, typename G, bool LOGIT>
 __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -568,21 +820,118 @@ __global__ __launch_bounds__(256) void step_kernel(RecArgs<T, G> a) {
   else store_part<T, V>(dst, p, left);
 }
 
+// The same backwards.  `before` holds the state in front of every step of a tile.
+template <typename T, typename G, typename S, bool EMIT, bool TINY>
+__device__ __forceinline__ void wide_tiles_grad(const RecArgs<T, G>& a, WidePairs<S::NW * S::TG, S::SLAB>& fw,
+                                                WidePairs<S::NW * S::TG, S::SLAB>& bw, float (*before)[S::SLAB], int64_t b,
+                                                int64_t n, int slab, int chunk, int64_t tile0, int64_t tile1, float& back,
+                                                float& prod, int& prod_e, bool& forgot) {
+  constexpr int V = S::V, L = S::L, GROUPS = S::NW * S::TG;
+  const Place<S, TINY> me(slab, a.slabs, a.D);
+  const int lane = me.lane, wave = me.wave, slot = me.slot, c = me.c, own = me.own, group = me.group, j = group * L;
+  back = EMIT && me.owner && a.d_last ? a.d_last[b * a.D + own] : 0.0f;
+  prod = 1.0f;
+  prod_e = 0;
+  forgot = false;
+  if (EMIT && me.owner) walk_chunks<T, G, false>(a, b, slab, chunk, own, back);
+#pragma unroll 1
+  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
+    const Rows rows = rows_of<S>(tile, n, a.reverse);
+    float carry = EMIT && me.owner ? a.carries[(b * a.tiles + tile) * a.D + own] : 0.0f;     // the state in front of the tile
+    float f[V], keep[V], x[V], in[V], d[V];
+    const auto step = [&](int k, bool with_x, bool with_d) {
+      Pack<T, V> px, pd;
+#pragma unroll
+      for (int i = 0; i < Pack<T, V>::WORDS; ++i) px.w[i] = pd.w[i] = 0;
+      if (with_x) px = load_step<S, T, TINY>(a.x + b * a.x_b, a.x_t, k, rows, a.reverse, c);
+      if (with_d && a.dh && k < rows.valid) pd = load_step<S, T, TINY>(a.dh + b * a.dh_b, a.dh_t, k, rows, a.reverse, c);
+      const Pack<G, V> pg = load_step<S, G, TINY>(a.g + b * a.g_b, a.g_t, k, rows, a.reverse, c);
+      step_of<T, G, V, false, false>(px, pg, k < rows.valid, f, keep, x, in);
+      unpack<T, V>(pd, d);
+      return reset_at(a, b, k, rows);
+    };
+    WidePair<V> p;
+#pragma unroll 1
+    for (int k = j; k < j + L; ++k) {
+      const bool r = step(k, EMIT, false);
+      p.add(f, in, r);
+    }
+    float C[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) C[v] = 0.0f;
+#pragma unroll 1
+    for (int k = j + L - 1; k >= j; --k) {
+      const bool r = step(k, false, true);
+#pragma unroll
+      for (int v = 0; v < V; ++v) C[v] = r ? 0.0f : f[v] * (d[v] + C[v]);
+    }
+    __syncthreads();        // the pairs of the tile before are done with
+    put_wide<V>(bw, group, slot, p.A, p.E, C, p.R);
+    if (EMIT) put_wide<V>(fw, group, slot, p.A, p.E, p.H, p.R);
+    __syncthreads();
+    if (wave == 0) {
+      walk_wide<GROUPS, S::SLAB, false, !EMIT>(bw, lane, back, prod, prod_e, forgot);
+      if (EMIT) walk_wide<GROUPS, S::SLAB, true, false>(fw, lane, carry, prod, prod_e, forgot);
+    }
+    if constexpr (EMIT) {
+      __syncthreads();
+      if (me.active) {
+        const int64_t base = b * a.T_ * a.D;
+        float s[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = fw.in[group][slot + v];
+#pragma unroll 1
+        for (int k = j; k < j + L; ++k) {
+          const bool r = step(k, true, false);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            before[k][slot + v] = r ? 0.0f : s[v];
+            s[v] = r ? in[v] : fmaf(f[v], s[v], in[v]);
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = bw.in[group][slot + v];
+#pragma unroll 1
+        for (int k = j + L - 1; k >= j; --k) {
+          const bool r = step(k, false, true), on = k < rows.valid;
+          float dx[V], dg[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float grad = d[v] + s[v];
+            dx[v] = on ? grad : 0.0f;
+            dg[v] = on ? grad * before[k][slot + v] : 0.0f;
+            s[v] = r ? 0.0f : f[v] * grad;
+          }
+          const int64_t at = tile * S::STEPS + k;
+          if (at < a.T_) {
+            put_step<S, T, TINY>(a.dx + base, at, n, a.reverse, c, a.D, pack<T, V>(dx));
+            put_step<S, G, TINY>(a.dg + base, at, n, a.reverse, c, a.D, pack<G, V>(dg));
+          }
+        }
+      }
+    }
+  }
+}
+
 // EMIT: gradients out; else the pair of a chunk's adjoint c_{t-1} = a_t (dh_t + c_t) alone.
 template <typename T, typename G, typename S, bool LOGIT, bool EMIT, bool TINY>
 __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, G> a) {
   constexpr int V = S::V, SLAB = S::SLAB, NW = S::NW, CL = S::CL, L = S::L;
   __shared__ Pairs<NW, SLAB> fw, bw;
+  __shared__ WidePairs<LOGIT ? 1 : NW * S::TG, SLAB> wide_fw, wide_bw;
+  __shared__ float before_steps[LOGIT || !EMIT ? 1 : S::STEPS][SLAB];
+  __shared__ int wave_grown[NW];      // decays: one above 1 in a wave's steps so far, or a wide chunk in front of them
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs;
   const int chunk = blockIdx.x / a.slabs + (EMIT ? 0 : 1);   // the first chunk's pair is not needed
   const int slot = (lane & (CL - 1)) * V;
-  const bool active = slab * SLAB + slot < a.D;
-  const int c = active ? channel_of<V, TINY>(slab * SLAB + slot, a.D) : 0;
+  const Slab mine = slab_of<S, LOGIT>(slab, a.slabs, a.D);
+  const bool active = slot < mine.width && mine.first + slot < a.D;
+  const int c = active ? channel_of<V, TINY>(mine.first + slot, a.D) : 0;
   // lane k of wave 0 carries the adjoint of this channel, lane k of the next wave (if there is one) its state
   constexpr int STATE_WAVE = NW > 1 ? 1 : 0;
-  const int own = channel_of<V, TINY>(slab * SLAB + lane / V * V, a.D) + lane % V;
-  const bool owns = lane < SLAB && slab * SLAB + lane / V * V < a.D && own < a.D;
+  const int own = channel_of<V, TINY>(mine.first + lane / V * V, a.D) + lane % V;
+  const bool owns = lane < mine.width && mine.first + lane / V * V < a.D && own < a.D;
   const bool owner = owns && wave == 0, stater = owns && wave == STATE_WAVE;
   const int j = (wave * S::TG + lane / CL) * L;
   const int64_t tile0 = chunk * a.chunk_tiles;
@@ -607,9 +956,10 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
     // the kept state in front of the tile
     float carry = EMIT && stater ? a.carries[(b * a.tiles + tile1 - 1) * a.D + own] : 0.0f;
     float back = EMIT && owner && a.d_last ? a.d_last[b * a.D + own] : 0.0f, prod = 1.0f;
-    bool forgot = false;
+    bool forgot = false, grown = false;
     if (EMIT && chunk + 1 < a.chunks)
-      through_chunks<T, G, S, false, TINY>(a, bw, b, chunk, lane, wave, slot, c, back);
+      through_chunks<T, G, S, !LOGIT, false, TINY>(a, bw, b, slab, chunk, lane, wave, slot, c, grown, back);
+    if constexpr (!LOGIT) wave_grown[wave] = grown;
     for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
       Tile<T, G, S> next;
       Pack<T, V> dnext[L];
@@ -631,7 +981,10 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
           for (int k = 0; k < Pack<T, V>::WORDS; ++k) cur.x[i].w[k] = 0;
       }
 
-      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets));
+      bool above = false;
+      if constexpr (!LOGIT) above = grows<G, V, L>(cur.g);
+      const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets) || above);
+      if (!LOGIT && !plain && __any(above)) wave_grown[wave] = 1;
       uint32_t resets = 0;
       float A[V], H[V], C[V], bA[V];     // this lane's pairs: forwards (A, H) and the adjoint's (bA, C)
       float e[L][V];                     // exp(-gate), or the decay itself: half the registers of a and 1 - a
@@ -765,14 +1118,18 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
 #pragma unroll
       for (int i = 0; i < L; ++i) dcur[i] = dnext[i];
     }
+    int prod_e = 0;
+    if constexpr (!LOGIT) {
+      if (__any(lane < NW && wave_grown[lane & (NW - 1)]))       // the same answer in every wave
+        wide_tiles_grad<T, G, S, EMIT, TINY>(a, wide_fw, wide_bw, before_steps, b, n, slab, chunk, tile0, tile1, back, prod,
+                                             prod_e, forgot);
+      if (b + gridDim.y < a.B) __syncthreads();                  // before the flags are written again
+    }
     if (owner) {
       if constexpr (EMIT) {
         if (a.dh0 && chunk == 0) a.dh0[b * a.D + own] = back;
       } else {
-        const int64_t o = b * a.chunks + chunk;
-        a.agg_a[o * a.D + own] = prod;
-        a.agg_h[o * a.D + own] = back;
-        if (lane == 0) a.agg_r[o] = forgot;
+        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, back, forgot);
       }
     }
   }
@@ -800,8 +1157,8 @@ Split split_of(int64_t B, int64_t T, int D, bool grad) {
   const int64_t pairs = s.chunks > 1 ? B * s.chunks * D * 4 : 0;
   s.agg_a = 0;
   s.agg_h = round_up(pairs, 256);
-  s.agg_r = 2 * s.agg_h;
-  s.bytes = s.chunks > 1 ? s.agg_r + round_up(B * s.chunks, 256) : 0;
+  s.agg_r = 3 * s.agg_h;      // the exponents lie between
+  s.bytes = s.chunks > 1 ? s.agg_r + round_up(B * s.chunks * s.slabs, 256) : 0;
   return s;
 }
 

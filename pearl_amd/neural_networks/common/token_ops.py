@@ -142,7 +142,7 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor] = 
         gate_logits=True:   h_t = a_t h_{t-1} + (1 - a_t) x_t,   a_t = sigmoid(gate_t)
         gate_logits=False:  h_t = gate_t h_{t-1} + x_t
 
-    ``gate`` has x's shape and its type, or float32 (decays close to one need it).  The state is float32
+    ``gate`` has x's shape and its type, or float32 (decays close to one need it); decays may be above one.  The state is float32
     throughout: ``initial_state`` (batch, channels; zeros if None) and the returned last state are
     float32, h is rounded to x's type.  ``resets`` (batch, time; bool) marks steps that begin an episode
     and ignore the state before them; ``lengths`` (batch) ends histories early: behind the end h is

@@ -1,11 +1,12 @@
 """The token-policy operators on the GPU at the edges of what their interfaces allow.  Definitions and
 bounds: tests/token_oracle.py."""
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import token_oracle as O
-from test_gpu_token_ops import DEV, DTYPES, IDS, check_log_probs, gen_of, np64, rnd
+from test_gpu_token_ops import DEV, DTYPES, IDS, check_log_probs, check_recurrence, gen_of, np64, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +153,103 @@ def test_a_state_written_in_place_is_known_to_autograd():
     leaf = torch.zeros(3, 8, device=DEV, requires_grad=True)
     with pytest.raises(RuntimeError):
         gated_recurrence_step(x, g, out_state=leaf)
+
+
+# ---------------------------------------------------------------------------- decays above one
+def growing_case(b, t, d, dtype, gate_dtype, key, resets=False, lengths=False):
+    """Channels whose products of decays leave the range of a float while their states stay inside it.
+    Kind 0: nothing but zeros meets growth.  1: zeros grow, then a decay of zero, then an ordinary history.
+    2: a state of 1e-30 grows by 1e50 and shrinks again.  3: factors of 1e10 and 1e-10 in turn.  4: ordinary."""
+    gen = gen_of(b, t, d, key)
+    half = t // 2
+    grow = 10.0 ** (50.0 / half) if half else 1.5
+    x, d_h = torch.randn(b, t, d, generator=gen), torch.randn(b, t, d, generator=gen)
+    g = 0.7 + 0.3 * torch.rand(b, t, d, generator=gen)
+    h0, d_last = torch.randn(b, d, generator=gen), torch.randn(b, d, generator=gen)
+    for c in range(d):
+        kind = (c + key) % 5
+        if kind == 0:
+            g[:, :, c], x[:, :, c], h0[:, c], d_h[:, :, c], d_last[:, c] = 1.5 * grow, 0.0, 0.0, 0.0, 0.0
+        if kind == 1:
+            g[:, :half, c], x[:, :half, c], h0[:, c] = grow * grow, 0.0, 0.0
+            g[:, half, c] = 0.0
+            d_h[:, :half, c] = 0.0
+        if kind == 2:
+            g[:, :half, c], g[:, half:, c] = grow, 1.0 / grow
+            x[:, :, c] = 0.0
+            h0[:, c] *= 1e-30
+            d_h[:, :, c] *= 1e-30
+            d_last[:, c] *= 1e-30
+        if kind == 3:
+            g[:, 0::2, c], g[:, 1::2, c] = 1e10, 1e-10
+    case = {"x": x.to(dtype), "g": g.to(gate_dtype), "h0": h0, "d_h": d_h.to(dtype), "d_last": d_last,
+            "resets": torch.rand(b, t, generator=gen) < 3.0 / t if resets else None,
+            "lengths": torch.randint(0, t + 1, (b,), generator=gen) if lengths else None}
+    return {k: None if v is None else v.to(DEV) for k, v in case.items()}
+
+
+# one step; one wave; one tile of half-width slabs; one tile and a cut of one tile a chunk; several tiles a
+# chunk; histories that are not cut; and a last slab of three channels after one of two fewer
+@pytest.mark.parametrize("b,t,d", [(2, 1, 10), (2, 24, 10), (1, 32, 37), (2, 100, 10), (1, 230, 10), (1, 2000, 10),
+                                   (26, 1300, 10), (140, 600, 5), (2, 24, 33), (2, 100, 65), (3, 300, 65), (1, 1500, 129)])
+@pytest.mark.parametrize("dtype,gate_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                              (torch.bfloat16, torch.bfloat16)], ids=["fp32", "bf16-fp32", "bf16"])
+def test_gated_recurrence_decays_above_one(b, t, d, dtype, gate_dtype):
+    with np.errstate(all="ignore"):
+        for key, (reverse, resets, lengths) in enumerate([(False, False, False), (True, True, True)]):
+            c = growing_case(b, t, d, dtype, gate_dtype, key, resets, lengths)
+            if reverse:
+                c["g"], c["x"], c["d_h"] = (c[k].flip(1).contiguous() for k in ("g", "x", "d_h"))
+            check_recurrence(c, False, reverse, dtype, gate_dtype, f"reverse {reverse}: ")
+
+
+def test_gated_recurrence_decays_above_one_leave_equal_bits():
+    """Channels beside those that grow, in the same workgroup and in the next: the same bits every time."""
+    from pearl_amd import gated_recurrence, gated_recurrence_grad
+    for t, d in ((24, 33), (100, 65), (1500, 129)):
+        gen = gen_of(t, d, 95)
+        x, d_h = rnd(gen, 2, t, d), rnd(gen, 2, t, d)
+        for at in (0, d - 10, d - 2, d - 1):
+            g = (0.9 + 0.05 * torch.rand(2, t, d, generator=gen)).to(DEV)
+            g[0, t // 3, at] = 1.5
+            first = None
+            for _ in range(6):
+                h, last, kept = gated_recurrence(x, g, gate_logits=False, keep=True)
+                out = [h, last, kept, *gated_recurrence_grad(x, g, kept, d_h, gate_logits=False)]
+                first = first or out
+                assert all(torch.equal(p, q) for p, q in zip(out, first)), (t, d, at)
+
+
+def test_gated_recurrence_decays_above_one_in_some_of_many_histories():
+    """More histories than a grid has rows, so that a workgroup walks several: each as if it were alone."""
+    from pearl_amd import gated_recurrence, gated_recurrence_grad
+    for t, d in ((20, 3), (40, 3), (130, 2)):
+        gen = gen_of(t, d, 96)
+        b = 65535 + 3000
+        x, d_h = rnd(gen, b, t, d), rnd(gen, b, t, d)
+        g = (0.9 + 0.05 * torch.rand(b, t, d, generator=gen)).to(DEV)
+        grow = torch.zeros(b, dtype=torch.bool)
+        grow[torch.randint(0, b, (2000,), generator=gen)] = True
+        grow[:1000] = True                       # followed by histories 65535 further on that do not grow,
+        grow[1000:2000], grow[66535:67535] = False, True      # and the other way round
+        g[grow.to(DEV)] *= 1.3
+        g[5, 3:9] = 0.0
+        def run(rows):
+            h, last, kept = gated_recurrence(x[rows], g[rows], gate_logits=False, keep=True)
+            return [h, last, *gated_recurrence_grad(x[rows], g[rows], kept, d_h[rows], gate_logits=False)]
+        whole = run(slice(None))
+        for rows in (slice(0, 3000), slice(30000, 33000), slice(65000, b)):
+            assert all(torch.equal(p[rows], q) for p, q in zip(whole, run(rows))), (t, d, rows)
+
+
+def test_gated_recurrence_decays_above_one_without_some_gradients():
+    from pearl_amd import gated_recurrence, gated_recurrence_grad
+    for t in (24, 100, 1500):
+        c = growing_case(2, t, 10, torch.float32, torch.float32, 1)
+        _, _, kept = gated_recurrence(c["x"], c["g"], c["h0"], gate_logits=False, keep=True)
+        zero, none = torch.zeros_like(c["d_h"]), torch.zeros_like(c["d_last"])
+        for given, full in (((None, c["d_last"]), (zero, c["d_last"])), ((c["d_h"], None), (c["d_h"], none)),
+                            ((None, None), (zero, none))):
+            for p, q in zip(gated_recurrence_grad(c["x"], c["g"], kept, *given, gate_logits=False),
+                            gated_recurrence_grad(c["x"], c["g"], kept, *full, gate_logits=False)):
+                assert torch.equal(p, q)
