@@ -102,3 +102,25 @@ def test_temperatures_whose_distances_pass_a_float_are_refused():
         with pytest.raises(ValueError):
             action_log_probs(torch.randn(2, 5), torch.zeros(2, dtype=torch.int64), temperature=far)
     assert 3.4028235e38 * 1.4427 / 2.0 ** 121 > 150 > 3.4028235e38 * 1.4427 / 1e38
+
+
+def test_the_cut_shapes_of_the_gpu_tests_reach_every_way_of_walking_pieces():
+    from pearl_amd import _native as N
+    from token_cuts import AT_ONCE, CUT_SHAPES, SLAB, cut
+    lib = N.lib()
+    up = lambda n: -(-n // 256) * 256  # noqa: E731
+    reached = set()
+    for b, t, d in CUT_SHAPES:
+        sizes = []
+        for direction in ("forward", "backward"):
+            tiles, per_piece, pieces = cut(b, t, d, direction)
+            assert pieces > 1
+            reached |= {(direction, "several tiles")} if per_piece > 1 else set()
+            reached |= {(direction, "several rounds")} if pieces - 1 > AT_ONCE[direction] else set()
+            reached |= {(direction, "both")} if per_piece > 1 and pieces - 1 > AT_ONCE[direction] else set()
+            # a factor, its exponent and a state per channel, and a byte per slab
+            sizes.append(3 * up(b * pieces * d * 4) + up(b * pieces * -(-d // SLAB)))
+        assert lib.pa_gated_recurrence_carries(b, t, d) == b * cut(b, t, d, "backward")[0] * d
+        assert lib.pa_gated_recurrence_scratch(b, t, d) == max(sizes), (b, t, d)
+    assert reached == {(direction, what) for direction in ("forward", "backward")
+                       for what in ("several tiles", "several rounds", "both")}
