@@ -1062,13 +1062,14 @@ int pa_concat_cols(const float* left, int32_t ldl, const float* right, int32_t l
 /* out[i, :] = scale * weight[tokens[i], :], rounded once: one_hot_action_representation_module.py:27-34
  * followed by a dense layer, without the one-hot matrix.  dtype (weight and out): PA_F32 / PA_BF16 /
  * PA_F16; tokens PA_I32 / PA_I64; weight rows ldw elements apart, out contiguous [n][dim].  Token -1
- * means none: a row of zeros, no gradient.  Any other token outside [0, vocab) gives a row of NaN. */
+ * means none: a row of zeros, no gradient.  Any other token outside [0, vocab) gives a row of NaN.  dim up to
+ * 2^30. */
 int pa_embed_tokens(const void* weight, int32_t dtype, int64_t ldw, int64_t vocab, int32_t dim,
                     const void* tokens, int32_t token_dtype, int64_t n, float scale, void* out,
                     int32_t device, void* stream);
 /* d_weight [vocab][dim] (written whole) = scale * sum over i with tokens[i] = v of d_out[i, :]: fp32
  * sums in index order, rounded once, the same bits for the same inputs.  Up to 2^26 tokens, 2^26
- * rows and 2^46 of their product, which the time grows with (a third of a second there).
+ * rows and 2^46 of their product, which the time grows with (a third of a second there); dim up to 2^25.
  * scratch: pa_embed_tokens_grad_scratch bytes, 256-byte aligned. */
 int64_t pa_embed_tokens_grad_scratch(int64_t n, int32_t dim, int32_t dtype);
 int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ldd, const void* tokens,

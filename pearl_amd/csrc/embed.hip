@@ -503,6 +503,7 @@ extern "C" int pa_embed_tokens(const void* weight, int32_t dtype, int64_t ldw, i
   PA_REQUIRE(n >= 0 && dim > 0 && vocab > 0 && vocab < 0xffffffffll && ldw >= dim, PA_ERR_INVALID,
              "pa_embed_tokens: bad shape (n %lld, vocab %lld, dim %d, ldw %lld)", (long long)n,
              (long long)vocab, dim, (long long)ldw);
+  PA_REQUIRE(dim <= (1 << 30), PA_ERR_UNSUPPORTED, "pa_embed_tokens: dim %d (up to 2^30)", dim);
   if (n == 0) return PA_OK;
   PA_REQUIRE(weight && tokens && out, PA_ERR_INVALID, "pa_embed_tokens: null pointer");
   PA_ON_DEVICE(device);
@@ -530,6 +531,8 @@ extern "C" int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ld
              "pa_embed_tokens_grad: %lld tokens times %lld rows (up to 2^46)", (long long)n, (long long)vocab);
   PA_REQUIRE(n >= 0 && dim > 0 && vocab > 0, PA_ERR_INVALID,
              "pa_embed_tokens_grad: bad shape (n %lld, vocab %lld, dim %d)", (long long)n, (long long)vocab, dim);
+  // a grid has 65535 rows of 1024 or 2048 columns
+  PA_REQUIRE(dim <= (1 << 25), PA_ERR_UNSUPPORTED, "pa_embed_tokens_grad: dim %d (up to 2^25)", dim);
   PA_REQUIRE(d_weight && (n == 0 || (d_out && tokens && scratch && ldd >= 0)), PA_ERR_INVALID,
              "pa_embed_tokens_grad: null pointer");
   PA_ON_DEVICE(device);

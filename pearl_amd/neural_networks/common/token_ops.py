@@ -82,8 +82,10 @@ def _embed(weight: Tensor, tokens: Tensor, scale: float) -> Tensor:
         raise ValueError(f"embed_tokens: weight has {weight.dim()} dimensions, not (vocab, dim)")
     code = dtype_code("embed_tokens", "weight", weight, FLOATS)
     index = dtype_code("embed_tokens", "tokens", tokens, INDICES)
-    on_one_gpu("embed_tokens", weight.device, tokens)
     vocab, dim = weight.shape
+    if dim > 2 ** 30:       # before the C entry, which takes 32 bits
+        raise NotImplementedError(f"embed_tokens: dim {dim} (up to 2^30)")
+    on_one_gpu("embed_tokens", weight.device, tokens)
     if weight.stride(1) != 1 or weight.stride(0) < dim:
         weight = weight.contiguous()
     tokens = tokens.contiguous()
@@ -96,15 +98,17 @@ def _embed(weight: Tensor, tokens: Tensor, scale: float) -> Tensor:
 
 def embed_tokens_grad(d_out: Tensor, tokens: Tensor, vocab: int, scale: float = 1.0) -> Tensor:
     """The gradient of ``embed_tokens`` with respect to its (vocab, dim) weight, in ``d_out``'s type.  Up to 2^26
-    tokens, 2^26 rows and 2^46 tokens times rows: the time grows with that product (0.06 ms at 2^33, 5.5 at 2^40)."""
+    tokens, 2^26 rows, 2^25 columns and 2^46 tokens times rows: the time grows with that product (0.06 ms at 2^33, 5.5 at 2^40)."""
     no_tangents("embed_tokens_grad", d_out)
     code = dtype_code("embed_tokens_grad", "d_out", d_out, FLOATS)
     index = dtype_code("embed_tokens_grad", "tokens", tokens, INDICES)
     if d_out.dim() < 1 or d_out.shape[:-1] != tokens.shape:
         raise ValueError(f"embed_tokens_grad: d_out has shape {tuple(d_out.shape)}, the tokens "
                          f"{tuple(tokens.shape)}")
-    on_one_gpu("embed_tokens_grad", d_out.device, tokens)
     n, dim = tokens.numel(), d_out.shape[-1]
+    if dim > 2 ** 25:
+        raise NotImplementedError(f"embed_tokens_grad: dim {dim} (up to 2^25)")
+    on_one_gpu("embed_tokens_grad", d_out.device, tokens)
     rows = d_out if d_out.dim() == 2 else d_out.reshape(n, dim)
     if rows.stride(1) != 1:
         rows = rows.contiguous()
@@ -142,9 +146,9 @@ def gated_recurrence(x: Tensor, gate: Tensor, initial_state: Optional[Tensor] = 
         gate_logits=True:   h_t = a_t h_{t-1} + (1 - a_t) x_t,   a_t = sigmoid(gate_t)
         gate_logits=False:  h_t = gate_t h_{t-1} + x_t
 
-    ``gate`` has x's shape and its type, or float32 (decays close to one need it); decays may be above one.  The state is float32
-    throughout: ``initial_state`` (batch, channels; zeros if None) and the returned last state are
-    float32, h is rounded to x's type.  ``resets`` (batch, time; bool) marks steps that begin an episode
+    ``gate`` has x's shape and its type, or float32 (decays close to one need it); decays may be above one.
+    The state is float32 throughout: ``initial_state`` (batch, channels; zeros if None) and the returned last
+    state are float32, h is rounded to x's type.  ``resets`` (batch, time; bool) marks steps that begin an episode
     and ignore the state before them; ``lengths`` (batch) ends histories early: behind the end h is
     zero, whatever x and gate hold there.  ``reverse`` runs from the last step to the first, as advantage
     sums do (a reset there marks the last step of an episode).
@@ -184,7 +188,8 @@ def _inputs(op: str, x: Tensor, gate: Tensor, resets: Optional[Tensor], lengths:
     code, gate_code = dtype_code(op, "x", x, FLOATS), dtype_code(op, "gate", gate, FLOATS)
     if gate_code != code and gate_code != N.PA_F32:
         raise TypeError(f"{op}: gate is {gate.dtype}, x is {x.dtype}: the gate has x's type or float32")
-    b, t, _ = x.shape
+    b, t, d = x.shape
+    _check_channels(op, d)
     if resets is not None:
         if resets.shape != (b, t) or resets.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"{op}: resets is {resets.dtype} {tuple(resets.shape)}, not bool {(b, t)}")
@@ -197,6 +202,11 @@ def _inputs(op: str, x: Tensor, gate: Tensor, resets: Optional[Tensor], lengths:
         # clamped before the cast, so that no length wraps around
         lengths = (lengths.clamp(0, t).to(torch.int32) if lengths.dtype == torch.int64 else lengths).contiguous()
     return code, gate_code, _rows(x), _rows(gate), resets, lengths
+
+
+def _check_channels(op: str, d: int) -> None:
+    if d >= 2 ** 21:        # rows of float32 gates 2^23 bytes long
+        raise NotImplementedError(f"{op}: {d} channels (fewer than 2^21)")
 
 
 def _check_state(op: str, name: str, state: Tensor, shape: Tuple[int, int]) -> Tensor:
@@ -311,6 +321,7 @@ def gated_recurrence_step(x: Tensor, gate: Tensor, state: Optional[Tensor] = Non
     if gate_code != code and gate_code != N.PA_F32:
         raise TypeError(f"{op}: gate is {gate.dtype}, x is {x.dtype}: the gate has x's type or float32")
     b, d = shape
+    _check_channels(op, d)
     if state is not None:
         state = _check_state(op, "state", state, shape)
     if resets is not None and (resets.shape != shape[:1] or resets.dtype not in (torch.bool, torch.uint8)):

@@ -55,6 +55,8 @@ def _inputs(op: str, logits: Tensor, actions: Tensor, mask: Optional[Tensor], te
         raise ValueError(f"{op}: temperature {temperature} (up to 2^121)")
     code, action_code = dtype_code(op, "logits", logits, FLOATS), dtype_code(op, "actions", actions, INDICES)
     width, rows = shape[-1], actions.numel()
+    if width >= 2 ** 31:
+        raise NotImplementedError(f"{op}: {width} actions (up to 2^31 - 1)")
     flat = logits if len(shape) == 2 else logits.reshape(rows, width)
     if flat.stride(1) != 1 and width > 1:
         flat = flat.contiguous()

@@ -124,3 +124,33 @@ def test_the_cut_shapes_of_the_gpu_tests_reach_every_way_of_walking_pieces():
         assert lib.pa_gated_recurrence_scratch(b, t, d) == max(sizes), (b, t, d)
     assert reached == {(direction, what) for direction in ("forward", "backward")
                        for what in ("several tiles", "several rounds", "both")}
+
+
+def test_rows_longer_than_the_c_entries_count_are_refused():
+    """Their lengths have 32 bits there: 2^32 + 4 columns would have been taken for 4."""
+    import pearl_amd as P
+    from pearl_amd import _native as N
+    tok, act = torch.tensor([0, 0]), torch.zeros(2, dtype=torch.int64)
+    for dim in (2 ** 30 + 1, 2 ** 31 + 4, 2 ** 32 + 4):
+        with pytest.raises(NotImplementedError):
+            P.embed_tokens(torch.zeros(1, 1).expand(1, dim), tok)
+    for dim in (2 ** 25 + 1, 2 ** 32 + 4):
+        with pytest.raises(NotImplementedError):
+            P.embed_tokens_grad(torch.zeros(1, 1).expand(2, dim), tok, 3)
+    for width in (2 ** 31, 2 ** 32 + 4):
+        with pytest.raises(NotImplementedError):
+            P.action_log_probs(torch.zeros(1, 1).expand(2, width), act)
+    x = torch.zeros(1, 1, 1).expand(1, 2, 2 ** 32 + 4)
+    with pytest.raises(NotImplementedError):
+        P.gated_recurrence(x, x)
+    with pytest.raises(NotImplementedError):
+        P.gated_recurrence_grad(x, x, torch.zeros(1))
+    with pytest.raises(NotImplementedError):
+        P.gated_recurrence_step(x[:, 0], x[:, 0])
+    lib = N.lib()
+    buf = C.cast((C.c_char * 4096)(), C.c_void_p).value
+    for dim in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.pa_embed_tokens(buf, N.PA_F32, 2 ** 32, 8, dim, buf, N.PA_I64, 2, 1.0, buf, 1000, None) == N.PA_ERR_UNSUPPORTED
+    for dim in (2 ** 25 + 1, 2 ** 31 - 1):
+        assert lib.pa_embed_tokens_grad(buf, N.PA_F32, 2 ** 32, buf, N.PA_I64, 2, 1.0, 8, dim, buf, buf, 1000,
+                                        None) == N.PA_ERR_UNSUPPORTED
