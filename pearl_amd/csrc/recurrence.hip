@@ -61,7 +61,7 @@ struct RecArgs {
   int reverse;
   int slabs, chunks; int64_t chunk_tiles, tiles;
   int64_t kept;                                  // states kept per history: the gradient's tiles
-  float* agg_a; float* agg_h; uint8_t* agg_r;    // [B][chunks][D], [B][chunks][slabs]: the chunks' pairs
+  float* agg_a; float* agg_h; uint8_t* agg_r;    // [B][chunks][D], [B][chunks] (decays: and [slabs]): the chunks' pairs
   T* h; float* last; float* carries;             // [B][T][D], [B][D] or null, [B][tiles][D] or null
   const T* dh; int64_t dh_b, dh_t;               // or null: zeros
   const float* d_last;                           // [B][D] or null
@@ -439,7 +439,8 @@ template <typename T, typename G>
 __device__ __forceinline__ int32_t* exponents(const RecArgs<T, G>& a) {
   return reinterpret_cast<int32_t*>(a.agg_h + (a.agg_h - a.agg_a));
 }
-// A chunk's pair is kept with its exponent; bit 0 of its byte: a reset, bit 1: some exponent is not 0.
+// A chunk's pair is kept with its exponent.  Bit 0 of its byte: a reset, which every slab of channels has alike;
+// bit 1: some exponent is not 0, which is a slab's own, so that decays have a byte for each.
 enum { CHUNK_RESET = 1, CHUNK_WIDE = 2 };
 template <typename T, typename G, bool LOGIT>
 __device__ __forceinline__ void put_chunk(const RecArgs<T, G>& a, int64_t b, int slab, int chunk, int lane, int own, float A,
@@ -449,7 +450,7 @@ __device__ __forceinline__ void put_chunk(const RecArgs<T, G>& a, int64_t b, int
   a.agg_h[o * a.D + own] = H;
   if constexpr (!LOGIT) exponents(a)[o * a.D + own] = E;
   const bool wide = !LOGIT && __any(E != 0);
-  if (lane == 0) a.agg_r[o * a.slabs + slab] = (reset ? CHUNK_RESET : 0) | (wide ? CHUNK_WIDE : 0);
+  if (lane == 0) a.agg_r[LOGIT ? o : o * a.slabs + slab] = (reset ? CHUNK_RESET : 0) | (wide ? CHUNK_WIDE : 0);
 }
 // A channel's state taken through the chunks in front of this one (UP; behind it, down), one after another.
 template <typename T, typename G, bool UP>
@@ -508,8 +509,8 @@ __device__ __forceinline__ void through_chunks(const RecArgs<T, G>& a, Pairs<S::
           A[v] = a.agg_a[o * a.D + c + v];
           H[v] = a.agg_h[o * a.D + c + v];
         }
-      const int flags = a.agg_r[o * a.slabs + slab];
-      R = flags & CHUNK_RESET;
+      const int flags = a.agg_r[DECAY ? o * a.slabs + slab : o];
+      R = DECAY ? flags & CHUNK_RESET : flags;
       if (DECAY && (flags & CHUNK_WIDE)) wide = true;
     }
     if (DECAY) grown = grown || __any(wide);
