@@ -359,12 +359,15 @@ __device__ __forceinline__ void join_waves(Pairs<NW, SLAB>& p, int lane, float& 
 
 // ---- decays above one --------------------------------------------------------------------------------
 // A product of many decays above one passes the range of a float though the states stay inside it: a state of
-// zero, or a small one, or decays that shrink again, and infinity times zero is no state.  Where a workgroup
-// has met a decay above 1 in size it walks its tiles a second time, with products kept as A 2^E, A between 1/2
-// and 1: every group of lanes takes its steps one after another, and one wave takes the groups.  A walk of its
-// own, behind the other and in rolled loops: the same arithmetic within the one loop cost histories without such
-// decays 8 to 14 % (registers: their loop uses all it may), the look at the decays costs 0 to 2 % (16 x 2048 x 1024
-// fp32 forwards 84.9 -> 86.8 us, bf16 35.7 both) and 1 us where a short history is cut.
+// zero, or a small one, or decays that shrink again, and infinity times zero is no state.  A workgroup counts how
+// far its channels' decays above one could take a product (the sum of their log2), and where that is further
+// than MAX_GROWTH it walks its tiles a second time, with products kept as A 2^E, A between 1/2 and 1: every group
+// of lanes takes its steps one after another, and one wave takes the groups.  A walk of its own, behind the other
+// and in rolled loops: the same arithmetic within the one loop cost histories without such decays 8 to 14 %
+// (registers: their loop uses all it may), the look at the decays costs 0 to 3 % (16 x 2048 x 1024 fp32 forwards
+// 85.0 -> 87.6 us, bf16 35.5 -> 36.2) and 1 us where a short history is cut.  The second walk takes twice to four
+// times the first (1 x 65536 x 512 bf16 forwards 60 us, with decays of 1.01 throughout 206).
+constexpr float MAX_GROWTH = 60.0f;      // 2^60: a state of up to 2^67 times such a product is still a float
 __device__ __forceinline__ void normalise(float& A, int& E) {
   const int e = E + __builtin_amdgcn_frexp_expf(A);      // zero, infinity and NaN: 0
   A = __builtin_amdgcn_frexp_mantf(A);
@@ -397,7 +400,24 @@ __device__ __forceinline__ bool grows(const Pack<G, V> (&g)[L]) {
   }
 }
 
-// The pairs of all groups of a tile and the states in front of them.
+// Adds up, for each of a lane's channels, how far decays above one could take a product.
+template <typename G, int V, int L>
+__device__ __forceinline__ void note_growth(float* growth, const Pack<G, V> (&g)[L], int first, int valid) {
+  float p[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] = 1.0f;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    float f[V];
+    unpack<G, V>(g[i], f);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (first + i < valid) p[v] *= fmaxf(fabsf(f[v]), 1.0f);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) growth[v] += __builtin_amdgcn_logf(p[v]);
+}
+// The pairs of all groups of a tile and the states in front of them.  (`in` holds the growth before a second walk.)
 template <int GROUPS, int SLAB>
 struct WidePairs {
   float A[GROUPS][SLAB], H[GROUPS][SLAB], in[GROUPS][SLAB];
@@ -439,19 +459,30 @@ template <typename T, typename G>
 __device__ __forceinline__ int32_t* exponents(const RecArgs<T, G>& a) {
   return reinterpret_cast<int32_t*>(a.agg_h + (a.agg_h - a.agg_a));
 }
+// What the growth of a workgroup's channels asks for.
+template <int GROUPS, int SLAB>
+__device__ __forceinline__ bool grows_past(const WidePairs<GROUPS, SLAB>& p, int lane, float limit) {
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < GROUPS; ++k) sum += p.in[k][lane & (SLAB - 1)];
+  return __any(!(sum <= limit));
+}
 // A chunk's pair is kept with its exponent.  Bit 0 of its byte: a reset, which every slab of channels has alike;
-// bit 1: some exponent is not 0, which is a slab's own, so that decays have a byte for each.
+// bit 1, a slab's own (so that decays have a byte for each): some exponent is not 0, or the product could be so large
+// that as many of them as there are chunks pass MAX_GROWTH.
 enum { CHUNK_RESET = 1, CHUNK_WIDE = 2 };
 template <typename T, typename G, bool LOGIT>
 __device__ __forceinline__ void put_chunk(const RecArgs<T, G>& a, int64_t b, int slab, int chunk, int lane, int own, float A,
-                                          int E, float H, bool reset) {
+                                          int E, float H, bool reset, bool large) {
   const int64_t o = b * a.chunks + chunk;
   a.agg_a[o * a.D + own] = A;
   a.agg_h[o * a.D + own] = H;
   if constexpr (!LOGIT) exponents(a)[o * a.D + own] = E;
-  const bool wide = !LOGIT && __any(E != 0);
+  const bool wide = !LOGIT && (large || __any(E != 0));
   if (lane == 0) a.agg_r[LOGIT ? o : o * a.slabs + slab] = (reset ? CHUNK_RESET : 0) | (wide ? CHUNK_WIDE : 0);
 }
+// What a wave of a decay kernel has met: decays above one among its steps; a wide chunk in front of its own.
+enum { GROWS = 1, AFTER_WIDE = 2 };
 // A channel's state taken through the chunks in front of this one (UP; behind it, down), one after another.
 template <typename T, typename G, bool UP>
 __device__ __forceinline__ void walk_chunks(const RecArgs<T, G>& a, int64_t b, int slab, int chunk, int own, float& state) {
@@ -649,7 +680,7 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
   constexpr int V = S::V, SLAB = S::SLAB, NW = S::NW, CL = S::CL, L = S::L;
   __shared__ Pairs<NW, SLAB> pairs;
   __shared__ WidePairs<LOGIT ? 1 : NW * S::TG, SLAB> wide;
-  __shared__ int wave_grown[NW];      // decays: one above 1 in a wave's steps so far, or a wide chunk in front of them
+  __shared__ int wave_grown[NW];      // decays: GROWS, AFTER_WIDE
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs, chunk = blockIdx.x / a.slabs;
   const int slot = (lane & (CL - 1)) * V;
@@ -678,7 +709,11 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
     float state = EMIT && owner && a.h0 ? a.h0[b * a.D + own] : 0.0f, prod = 1.0f;
     bool forgot = false, grown = false;
     if (EMIT && chunk) through_chunks<T, G, S, !LOGIT, true, TINY>(a, pairs, b, slab, chunk, lane, wave, slot, c, grown, state);
-    if constexpr (!LOGIT) wave_grown[wave] = grown;
+    if constexpr (!LOGIT) {
+      wave_grown[wave] = grown ? AFTER_WIDE : 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) wide.in[j / L][slot + v] = 0.0f;
+    }
     for (int64_t tile = tile0; tile < tile1; ++tile) {
       Tile<T, G, S> next;
       const Rows after = rows_of<S>(tile + 1 < tile1 ? tile + 1 : tile, n, a.reverse);
@@ -690,7 +725,11 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       bool above = false;
       if constexpr (!LOGIT) above = grows<G, V, L>(cur.g);
       const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets) || above);
-      if (!LOGIT && !plain && __any(above)) wave_grown[wave] = 1;
+      if constexpr (!LOGIT)
+        if (!plain && __any(above)) {
+          wave_grown[wave] |= GROWS;
+          note_growth<G, V, L>(&wide.in[j / L][slot], cur.g, j, rows.valid);
+        }
       uint32_t resets = 0;
       float A[L][V], H[L][V], sA[V], sH[V];
       bool sR = false;
@@ -768,8 +807,16 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       rows = after;
     }
     int prod_e = 0;
+    bool large = false;
     if constexpr (!LOGIT) {
-      if (__any(lane < NW && wave_grown[lane & (NW - 1)]))       // the same answer in every wave
+      // the same answers in every wave: each looks at all of them, and at all channels
+      const int grew = lane < NW ? wave_grown[lane & (NW - 1)] : 0;
+      bool again = __any(grew & AFTER_WIDE);
+      if (__any(grew & GROWS)) {
+        again = again || grows_past(wide, lane, MAX_GROWTH);
+        if (!EMIT) large = grows_past(wide, lane, MAX_GROWTH / a.chunks);
+      }
+      if (again)
         wide_tiles<T, G, S, EMIT, TINY>(a, wide, b, n, slab, chunk, tile0, tile1, state, prod, prod_e, forgot);
       if (b + gridDim.y < a.B) __syncthreads();                  // before the flags are written again
     }
@@ -777,7 +824,7 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_kernel(RecArgs<T, G> a)
       if constexpr (EMIT) {
         if (a.last && chunk == a.chunks - 1) a.last[b * a.D + own] = state;
       } else {
-        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, state, forgot);
+        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, state, forgot, large);
       }
     }
   }
@@ -921,7 +968,7 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
   __shared__ Pairs<NW, SLAB> fw, bw;
   __shared__ WidePairs<LOGIT ? 1 : NW * S::TG, SLAB> wide_fw, wide_bw;
   __shared__ float before_steps[LOGIT || !EMIT ? 1 : S::STEPS][SLAB];
-  __shared__ int wave_grown[NW];      // decays: one above 1 in a wave's steps so far, or a wide chunk in front of them
+  __shared__ int wave_grown[NW];      // decays: GROWS, AFTER_WIDE
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slab = blockIdx.x % a.slabs;
   const int chunk = blockIdx.x / a.slabs + (EMIT ? 0 : 1);   // the first chunk's pair is not needed
@@ -960,7 +1007,11 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
     bool forgot = false, grown = false;
     if (EMIT && chunk + 1 < a.chunks)
       through_chunks<T, G, S, !LOGIT, false, TINY>(a, bw, b, slab, chunk, lane, wave, slot, c, grown, back);
-    if constexpr (!LOGIT) wave_grown[wave] = grown;
+    if constexpr (!LOGIT) {
+      wave_grown[wave] = grown ? AFTER_WIDE : 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) wide_bw.in[j / L][slot + v] = 0.0f;
+    }
     for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
       Tile<T, G, S> next;
       Pack<T, V> dnext[L];
@@ -985,7 +1036,11 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
       bool above = false;
       if constexpr (!LOGIT) above = grows<G, V, L>(cur.g);
       const bool plain = rows.valid == S::STEPS && !__any(any_reset(cur.resets) || above);
-      if (!LOGIT && !plain && __any(above)) wave_grown[wave] = 1;
+      if constexpr (!LOGIT)
+        if (!plain && __any(above)) {
+          wave_grown[wave] |= GROWS;
+          note_growth<G, V, L>(&wide_bw.in[j / L][slot], cur.g, j, rows.valid);
+        }
       uint32_t resets = 0;
       float A[V], H[V], C[V], bA[V];     // this lane's pairs: forwards (A, H) and the adjoint's (bA, C)
       float e[L][V];                     // exp(-gate), or the decay itself: half the registers of a and 1 - a
@@ -1120,8 +1175,16 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
       for (int i = 0; i < L; ++i) dcur[i] = dnext[i];
     }
     int prod_e = 0;
+    bool large = false;
     if constexpr (!LOGIT) {
-      if (__any(lane < NW && wave_grown[lane & (NW - 1)]))       // the same answer in every wave
+      // the same answers in every wave: each looks at all of them, and at all channels
+      const int grew = lane < NW ? wave_grown[lane & (NW - 1)] : 0;
+      bool again = __any(grew & AFTER_WIDE);
+      if (__any(grew & GROWS)) {
+        again = again || grows_past(wide_bw, lane, MAX_GROWTH);
+        if (!EMIT) large = grows_past(wide_bw, lane, MAX_GROWTH / a.chunks);
+      }
+      if (again)
         wide_tiles_grad<T, G, S, EMIT, TINY>(a, wide_fw, wide_bw, before_steps, b, n, slab, chunk, tile0, tile1, back, prod,
                                              prod_e, forgot);
       if (b + gridDim.y < a.B) __syncthreads();                  // before the flags are written again
@@ -1130,7 +1193,7 @@ __global__ __launch_bounds__(S::NW * 64) void recurrence_grad_kernel(RecArgs<T, 
       if constexpr (EMIT) {
         if (a.dh0 && chunk == 0) a.dh0[b * a.D + own] = back;
       } else {
-        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, back, forgot);
+        put_chunk<T, G, LOGIT>(a, b, slab, chunk, lane, own, prod, prod_e, back, forgot, large);
       }
     }
   }

@@ -253,3 +253,19 @@ def test_gated_recurrence_decays_above_one_without_some_gradients():
             for p, q in zip(gated_recurrence_grad(c["x"], c["g"], kept, *given, gate_logits=False),
                             gated_recurrence_grad(c["x"], c["g"], kept, *full, gate_logits=False)):
                 assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("b,t,d", [(2, 30, 9), (2, 120, 9), (3, 250, 65), (1, 2000, 9), (26, 1300, 9), (140, 600, 5)])
+def test_gated_recurrence_decays_a_little_above_one(b, t, d, dtype):
+    """Products from hardly above one to past 2^60, by channel: some workgroups walk their tiles twice, some chunks
+    are joined one after another, others are not."""
+    gen = gen_of(b, t, d, 97)
+    for reverse in (False, True):
+        bits = torch.rand(b, 1, d, generator=gen) * 120.0 / t * torch.randint(0, 2, (b, 1, d), generator=gen)
+        up = (torch.rand(b, t, d, generator=gen) < 0.5).double()
+        g = torch.exp2(bits * (2 * up - 1))                    # as many steps up as down: the states stay in range
+        c = {"x": rnd(gen, b, t, d, dtype=dtype), "g": g.float().to(DEV), "h0": rnd(gen, b, d), "lengths": None,
+             "resets": (torch.rand(b, t, generator=gen) < 2.0 / t).to(DEV) if reverse else None,
+             "d_h": rnd(gen, b, t, d, dtype=dtype), "d_last": rnd(gen, b, d)}
+        check_recurrence(c, False, reverse, dtype, torch.float32, f"reverse {reverse}: ")
