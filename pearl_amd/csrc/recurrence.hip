@@ -12,13 +12,14 @@
 // 32 lanes of two channels side by side in a row, two groups of 8 consecutive steps per wave, waves behind
 // one another in time.  Each lane scans its own steps, the groups are joined by one lane shuffle, the
 // waves through LDS by one wave, which carries the state on, while the next tile's loads are already under
-// way.  Every input is read once and every output written once.  The state is fp32 throughout; only the
-// stored h is rounded to the input's type.
+// way.  Every output is written once and every input read once, but for a workgroup's last prefetch, which finds
+// no further tile and loads the last one again (a gradient without d_h loads rows of x in its place).  The state
+// is fp32 throughout; only the stored h is rounded to the input's type.
 //
 // Two channels a lane, because what a step costs beside its loads is the joining: with eight a lane (16-byte
-// loads) the tile needs three shuffles of 16 values (61 us against 49 at 16 x 2048 x 1024 bf16, 201 MB; the
-// same accesses without arithmetic take 31).  Forwards 21 VALU instructions a value, backwards 40; the rest
-// of the time is the tile's two barriers.
+// loads) the tile needs three shuffles of 16 values (61 us against 49 at 16 x 2048 x 1024 bf16, 201 MB, which a
+// copy moves in 39).  Forwards 21 VALU instructions a value, backwards 40; the rest of the time is the tile's
+// two barriers.
 //
 // Where batch x channels give too few workgroups, the steps are cut into chunks: a first launch
 // composes each chunk's pair, the second starts every chunk from the composition of those before it
@@ -68,8 +69,10 @@ struct RecArgs {
   T* dx; G* dg; float* dh0;                      // dh0 or null
 };
 
-// a and 1 - a of a logit, both to a few ulp, also where one of them is tiny.  Below -87 a stays at 2e-38,
-// the smallest normal number (1 / a would overflow); NaN stays NaN (maximum, not fmax).
+// a and 1 - a of a logit, each to its own size also where it is tiny: the smaller is off by up to about
+// (|z| + 4) 2^-24 of itself (the exponential's argument is rounded once), the larger by a few 2^-24.  Below -87
+// a stays at 1.6e-38: a little further down the exponential would be infinite, and 1 - a infinity times zero.
+// NaN stays NaN (maximum, not fmax).
 __device__ __forceinline__ float exp_minus(float z) {
   return __builtin_amdgcn_exp2f(-1.44269504088896340736f * __builtin_elementwise_maximum(z, -87.0f));
 }
