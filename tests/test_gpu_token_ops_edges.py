@@ -269,3 +269,37 @@ def test_gated_recurrence_decays_a_little_above_one(b, t, d, dtype):
              "resets": (torch.rand(b, t, generator=gen) < 2.0 / t).to(DEV) if reverse else None,
              "d_h": rnd(gen, b, t, d, dtype=dtype), "d_last": rnd(gen, b, d)}
         check_recurrence(c, False, reverse, dtype, torch.float32, f"reverse {reverse}: ")
+
+
+@pytest.mark.parametrize("b,t,d", [(2, 30, 8), (2, 120, 8), (1, 900, 8), (30, 700, 8)])
+def test_gated_recurrence_half_precision_decays_above_one(b, t, d):
+    """Of eight channels: zeros that meet growth; the same, forgotten by a decay of zero; a state of 1e-30 that grows by
+    2^100 and shrinks again; ones; minus ones; ordinary ones.  What float16 cannot hold is left out of its gradients."""
+    half = t // 2
+    grow = 2.0 ** (100.0 / half)
+    gen = gen_of(b, t, d, 98)
+    x, d_h = torch.randn(b, t, d, generator=gen), torch.randn(b, t, d, generator=gen)
+    g = 0.7 + 0.3 * torch.rand(b, t, d, generator=gen)
+    h0, d_last = torch.randn(b, d, generator=gen), torch.randn(b, d, generator=gen)
+    g[..., 0], x[..., 0], h0[:, 0], d_h[..., 0], d_last[:, 0] = 40.0, 0.0, 0.0, 0.0, 0.0
+    g[:, :half, 1], g[:, half, 1], x[:, :half, 1], h0[:, 1], d_h[:, :half, 1] = 60000.0, 0.0, 0.0, 0.0, 0.0
+    g[:, :half, 2], g[:, half:, 2], x[..., 2], d_h[..., 2] = grow, 1.0 / grow, 0.0, 0.0
+    h0[:, 2] *= 1e-30
+    d_last[:, 2] *= 1e-30
+    g[..., 3], g[..., 4] = 1.0, -1.0
+    for reverse in (False, True):
+        turn = (lambda v: v.flip(1)) if reverse else (lambda v: v)
+        c = {"x": turn(x).half().to(DEV), "g": turn(g).half().to(DEV), "h0": h0.to(DEV), "d_h": turn(d_h).half().to(DEV),
+             "d_last": d_last.to(DEV), "resets": None, "lengths": None}
+        from pearl_amd import gated_recurrence, gated_recurrence_grad
+        want = O.recurrence(np64(c["x"]), np64(c["g"]), np64(c["h0"]), None, None, False, reverse, np64(c["d_h"]),
+                            np64(c["d_last"]))
+        # Of the third channel the adjoint, 1e-30 behind the last step, is 1e-30 2^-100 in front of the shrinking
+        # half: a float32 holds nothing below 2^-149, so whatever walks the steps may be off by half of that there,
+        # and the growing half takes it 2^100 further, to 2^-50 (decays rounded to float16: a factor of 2 at most).
+        want["d_h0"][1][:, 2] += 2.0 ** -49
+        h, last, kept = gated_recurrence(c["x"], c["g"], c["h0"], gate_logits=False, reverse=reverse, keep=True)
+        out = gated_recurrence_grad(c["x"], c["g"], kept, c["d_h"], c["d_last"], gate_logits=False, reverse=reverse)
+        for name, got in zip(("h", "last", "d_x", "d_g", "d_h0"), (h, last, *out)):
+            kind = torch.float32 if name in ("last", "d_h0") else torch.float16
+            O.check(got, *want[name], kind, f"reverse {reverse}: {name}")
