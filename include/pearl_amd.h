@@ -1081,7 +1081,9 @@ int pa_embed_tokens_grad(const void* d_out, int32_t dtype, int64_t ldd, const vo
  *   gate_logits = 1:  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(g_t)
  * The state is fp32; h is rounded to the input's type.  g_t may be of any size: products of decays above one are
  * kept with an exponent of their own, so a state is what its steps make of it as long as it, and the sum of the
- * sizes of what it adds up, stays inside the range of a float.  Strides in elements, channels adjacent. */
+ * sizes of what it adds up, stays inside the range of a float.  The history is scanned in parallel: what a product of
+ * factors below 2^-126 leaves of an earlier state is rounded as a float that small is, and below 2^-149 it is 0.
+ * Strides in elements, channels adjacent. */
 typedef struct pa_recurrence_args {
   int32_t device;
   int32_t dtype;              /* of x, h, d_h, d_x: PA_F32 / PA_BF16 / PA_F16               */
